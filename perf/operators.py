@@ -219,12 +219,20 @@ def _library():
     return obsmoe
 
 
+_contexts = {}  # one for each shape of cache, as a program keeps one for its model
+
+
 def _prepare_own(s):
     """The context with its workspace, and the caches' descriptors: what a program makes once."""
     lib, c = _library(), s.case
-    s.ctx = lib.MoeContext(lib.MoeShape(hidden=2048, inter=256, n_experts=16, top_k=4, n_layers=1, max_tokens=1))
-    s.ctx.paged_init(n_heads=c["heads"], n_kv_heads=c["kv_heads"], head_dim=c["head_dim"], page_size=c["page"], max_seqs=c["n"],
-                     max_kv_len=s.max_len, dtype=c["type"], weights=c["op"] == "decode" and c["weights"])
+    plan = dict(n_heads=c["heads"], n_kv_heads=c["kv_heads"], head_dim=c["head_dim"], page_size=c["page"], max_seqs=c["n"],
+                max_kv_len=s.max_len, dtype=c["type"], weights=c["op"] == "decode" and c["weights"])
+    key = tuple(plan.values())
+    if key not in _contexts:
+        ctx = lib.MoeContext(lib.MoeShape(hidden=2048, inter=256, n_experts=16, top_k=4, n_layers=1, max_tokens=1))
+        ctx.paged_init(**plan)
+        _contexts[key] = ctx
+    s.ctx = _contexts[key]
     s.kv = lib.PagedKV(s.k, s.v, s.table, s.len)
     if c["op"] == "evict":
         s.to_kv = lib.PagedKV(s.to_k, s.to_v, s.to_table, s.to_len)
