@@ -111,6 +111,40 @@ typedef struct obs_attn_config {
     float rope_theta;    /* 1e7 */
 } obs_attn_config;
 
+/* Element types of the paged cache's keys, values, queries and outputs. */
+enum obs_dtype { OBS_DTYPE_BF16 = 0, OBS_DTYPE_F16 = 1 };
+
+/* The paged key/value cache's shape (obs_paged_init). */
+typedef struct obs_paged_config {
+    int32_t n_heads;     /* query heads */
+    int32_t n_kv_heads;  /* key/value heads; n_heads a multiple of it, at most 16 times it */
+    int32_t head_dim;    /* <= 128, a multiple of 8 */
+    int32_t page_size;   /* positions per page, 1..1024 */
+    int32_t max_seqs;    /* sequences of one call (<= 65535) */
+    int32_t max_kv_len;  /* positions of one sequence (<= 1048576) */
+    int32_t dtype;       /* enum obs_dtype */
+    int32_t weights;     /* != 0: decode steps may add up attention weights (workspace for their scores) */
+} obs_paged_config;
+
+/* One layer's paged cache, memory the caller owns (device pointers).  Position j
+ * of sequence s, head h, is the row of head_dim elements at
+ *   k + block_table[s * table_stride + j / page_size] * page_stride
+ *     + (j % page_size) * slot_stride + h * head_stride
+ * (v likewise); strides in elements, multiples of 8; k and v 16-byte aligned. */
+typedef struct obs_paged_kv {
+    void* k;
+    void* v;
+    const int32_t* block_table;  /* [n_seqs][table_stride] page ids in [0, n_pages) */
+    const int32_t* kv_len;       /* [n_seqs] positions held */
+    int64_t page_stride;
+    int64_t slot_stride;
+    int64_t head_stride;
+    int32_t n_seqs;
+    int32_t n_pages;
+    int32_t table_stride;        /* entries from one sequence's row of block_table to the next */
+    int32_t table_pages;         /* entries of a row in use: room for table_pages * page_size positions */
+} obs_paged_kv;
+
 /* ---------------------------------------------------------------- context */
 int obs_abi_version(void);
 /* Replaces ObsidianExecutor::new (src/executor.rs:39-58) and the expert pools
@@ -196,6 +230,69 @@ int obs_attn_forward(obs_ctx* ctx, int layer, const uint16_t* x, uint16_t* out, 
 /* Copies cache positions [pos0, pos0 + n) of one sequence and layer: k and v
  * (either may be NULL) bf16 [n_kv_heads][n][head_dim], device memory. */
 int obs_kv_read(obs_ctx* ctx, int layer, int seq, int pos0, int n, uint16_t* k, uint16_t* v, void* stream);
+
+/* ------------------------------------------------ the paged key/value cache */
+/* No counterpart in the reference, whose cache is one dense buffer per layer
+ * (src/kv_cache.rs:15-24).  The caller owns the pools, the page tables and the
+ * lengths; a call is given one layer's cache (obs_paged_kv).  Tables and lengths
+ * are read on the device, in stream order, so a captured CUDA graph serves
+ * growing sequences.  A page id outside the pool or a length beyond the table
+ * (or max_kv_len, or a weights row) is refused on the device: such rows are left
+ * out and obs_check_device reports OBS_ERR_INVALID.
+ *
+ * obs_paged_init: the shape that the calls below take and their workspace, once
+ * per context (independent of obs_attn_init and of the number of layers). */
+int obs_paged_init(obs_ctx* ctx, const obs_paged_config* cfg);
+/* k and v rows t = 0 .. T-1 ([n_kv_heads][head_dim] each, rows row_stride elements
+ * apart) to position slot[t] of sequence seq[t] (device int32 [T]); the (sequence,
+ * position) pairs of one call are distinct.  A row outside the cache is refused on
+ * the device (OBS_ERR_INVALID from obs_check_device).  kv_len is not read. */
+int obs_paged_append(obs_ctx* ctx, const obs_paged_kv* kv, const void* k, const void* v, int64_t row_stride,
+                     const int32_t* seq, const int32_t* slot, int T, void* stream);
+/* Attention of one new token per sequence: q row s ([n_heads][head_dim], rows
+ * q_stride elements apart) at position i = kv_len[s] - 1 sees the positions j <= i
+ * with window == 0 or i - j < window or j < n_sink;
+ *   out[s][h] = sum_j p_j v_j,  p = softmax_j(scale * q . k_j)   (scale 0: 1/sqrt(head_dim))
+ * out [n_seqs][n_heads][head_dim].  A sequence of length 0 gives zeros.  Sums and
+ * the softmax in fp32, one rounding at the end (p is rounded to the element type
+ * for the product with v).  weights (optional, fp32 [n_seqs][n_kv_heads][w_stride]):
+ * weights[s][g][j] += the p_j of KV head g's query heads, summed. */
+int obs_paged_decode(obs_ctx* ctx, const obs_paged_kv* kv, const void* q, int64_t q_stride, void* out, int window,
+                     int n_sink, float scale, float* weights, int w_stride, void* stream);
+/* Attention of the new tokens of several prompts (or chunks of them): rows
+ * q_start[s] .. q_start[s+1] - 1 of q and out (device int32 [n_seqs + 1], from 0 to
+ * T, not decreasing) are sequence s's last positions, the last of them kv_len[s] - 1
+ * (their keys and values already appended); each sees what a decode at its position
+ * would see.  A row with nothing to see (more rows than kv_len[s]) gives zeros. */
+int obs_paged_prefill(obs_ctx* ctx, const obs_paged_kv* kv, const void* q, int64_t q_stride, void* out,
+                      const int32_t* q_start, int T, int window, int n_sink, float scale, void* stream);
+/* Eviction by accumulated attention weight, per sequence and KV head: of n =
+ * kv_len[s] positions all stay if n <= budget, else the first n_sink, the last
+ * n_recent and those with the largest weights of the rest, budget in all (equal
+ * weights: the lowest position; NaN counts as the lowest).  The kept rows move in
+ * their order to positions 0, 1, ... of dst; kept [n_seqs][n_kv_heads][budget]
+ * receives their old positions (-1 past the end) and new_len [n_seqs] min(n,
+ * budget).  weights_dst (optional, same shape as weights) receives the kept
+ * positions' weights, zeros after them.  dst is either kv itself (same pools and
+ * table; weights_dst may then be weights) or holds pages that kv does not hold;
+ * in place, no page may belong to two sequences.  dst->kv_len is not read;
+ * new_len may not be kv->kv_len. */
+int obs_paged_evict(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_kv* dst, const float* weights,
+                    float* weights_dst, int w_stride, int budget, int n_sink, int n_recent, int32_t* kept,
+                    int32_t* new_len, void* stream);
+/* obs_attn_forward over a paged cache: the same projections, norms and RoPE at
+ * pos[t], K and V appended at position slot[t] of sequence seq[t] (slot differs
+ * from pos after an eviction), then obs_paged_decode (q_start NULL: T = n_seqs,
+ * token t is sequence t's; weights optional) or obs_paged_prefill (q_start as
+ * there), the o projection and the residual.  kv->kv_len already counts this call's
+ * tokens.  Needs obs_attn_init, obs_load_attn and obs_paged_init of the same heads
+ * and head_dim in bf16; the dense caches are not used. */
+int obs_paged_attn_forward(obs_ctx* ctx, int layer, const obs_paged_kv* kv, const uint16_t* x, uint16_t* out, int T,
+                           const int32_t* seq, const int32_t* pos, const int32_t* slot, const int32_t* q_start,
+                           int window, int n_sink, float* weights, int w_stride, void* stream);
+/* As obs_struct_layout: sizeof(obs_paged_config), the offsets of its 8 fields,
+ * sizeof(obs_paged_kv), the offsets of its 11 fields (21 values). */
+int obs_paged_struct_layout(int32_t* out, int n);
 
 /* ------------------------------------------------------ the MoE layer path */
 /* out = [residual +] sum_k w_k * expert_k(x): router -> top-k -> dispatch ->

@@ -40,7 +40,9 @@ __device__ __forceinline__ void rope_pair(float x0, float x1, float c, float s, 
 // and k (nkv heads): grid (T, nq + nkv), 128 threads.  qkv: fp32 projections
 // [T][nq*hd + 2*nkv*hd] (q | k | v).  The head's rms in rmsnorm.metal's order
 // (256 "threads" strided over hd, halving tree) -- here 128 threads carry the
-// first 128 partials and the upper 128 are zero, which is the same sum.
+// first 128 partials and the upper 128 are zero, which is the same sum.  kv_rows:
+// K and V go to row t of kcache / vcache ([T][nkv][hd], for a paged cache's append)
+// instead of the sequence's cache.
 __global__ void __launch_bounds__(kAttnThreads) k_qk_norm_rope(const float* qkv, int T, int nq, int nkv,
                                                                int hd, const uint16_t* __restrict__ qn,
                                                                const uint16_t* __restrict__ kn, float eps,
@@ -48,7 +50,7 @@ __global__ void __launch_bounds__(kAttnThreads) k_qk_norm_rope(const float* qkv,
                                                                const int32_t* seq,
                                                                const int32_t* pos,
                                                                uint16_t* __restrict__ qout, uint16_t* kcache,
-                                                               uint16_t* vcache, int n_seqs, int* err) {
+                                                               uint16_t* vcache, int n_seqs, int* err, int kv_rows) {
     pdl_begin();
     __shared__ float sq[256];
     __shared__ float sx[128];
@@ -84,13 +86,13 @@ __global__ void __launch_bounds__(kAttnThreads) k_qk_norm_rope(const float* qkv,
             uint16_t* dst = qout + ((size_t)t * nq + h) * hd;
             dst[l] = o0, dst[l + half] = o1;
         } else {
-            uint16_t* dst = kcache + (((size_t)s_id * nkv + hh) * max_seq + p) * hd;
+            uint16_t* dst = kcache + (kv_rows ? (size_t)t * nkv + hh : ((size_t)s_id * nkv + hh) * max_seq + p) * hd;
             dst[l] = o0, dst[l + half] = o1;
         }
     }
     if (!isq && l < hd) {  // v: the projection rounded to bf16, no norm, no rotation
         const float* vs = qkv + (size_t)t * width + (size_t)(nq + nkv) * hd + (size_t)hh * hd;
-        vcache[(((size_t)s_id * nkv + hh) * max_seq + p) * hd + l] = f2bf(vs[l]);
+        vcache[(kv_rows ? (size_t)t * nkv + hh : ((size_t)s_id * nkv + hh) * max_seq + p) * hd + l] = f2bf(vs[l]);
     }
 }
 
@@ -241,11 +243,12 @@ __global__ void k_residual_add(const uint16_t* x, const float* o, size_t n,
 cudaError_t launch_qk_norm_rope(const float* qkv, int T, int nq, int nkv, int hd, const uint16_t* qn,
                                 const uint16_t* kn, float eps, const float* rope_cs, int max_seq, const int32_t* seq,
                                 const int32_t* pos, uint16_t* qout, uint16_t* kcache, uint16_t* vcache, int n_seqs,
-                                int* err, cudaStream_t st) {
+                                int* err, cudaStream_t st, int kv_rows) {
     if (T <= 0) return cudaSuccess;
     if (hd > 128 || hd % 2) return cudaErrorInvalidValue;
     const cudaError_t e = launch_pdl(k_qk_norm_rope, dim3(T, nq + nkv), dim3(kAttnThreads), 0, st, qkv, T, nq, nkv,
-                                     hd, qn, kn, eps, rope_cs, max_seq, seq, pos, qout, kcache, vcache, n_seqs, err);
+                                     hd, qn, kn, eps, rope_cs, max_seq, seq, pos, qout, kcache, vcache, n_seqs, err,
+                                     kv_rows);
     if (e != cudaSuccess) return e;
     return cudaGetLastError();
 }

@@ -115,6 +115,8 @@ struct obs_ctx {
     uint16_t* a_out = nullptr;  // [max_tokens][nq hd]
     float* a_o = nullptr;       // [max_tokens][H]
     float* a_part = nullptr;    // the attention splits' partial sums (sdpa_part_floats)
+    uint16_t* a_kv = nullptr;   // [2][max_tokens][nkv hd] K and V rows on their way into a paged cache
+    PagedState* paged = nullptr;  // obs_paged_init
     size_t ep_bytes = 0;
     bool ep_connected = false;
     EpArgs ep{};
@@ -177,6 +179,7 @@ static int fail(obs_ctx* c, int code, const std::string& msg);
 namespace obs {
 void ctx_shape(const obs_ctx* ctx, int* E, int* H, int* I) { *E = ctx->sh.E, *H = ctx->sh.H, *I = ctx->sh.I; }
 int ctx_fail(obs_ctx* ctx, int code, const char* msg) { return fail(ctx, code, msg ? msg : ""); }
+CtxParts ctx_parts(obs_ctx* ctx) { return {ctx->device, ctx->num_sms, ctx->err_flag, ctx->wait_ns, &ctx->paged}; }
 }  // namespace obs
 
 static size_t layer_weight_bytes(const Shape& s, int E_local) {
@@ -395,6 +398,7 @@ extern "C" int obs_destroy(obs_ctx* ctx) {
     for (auto& a : ctx->attn)
         if (a.mem) cudaFree(a.mem);
     if (ctx->attn_scratch) cudaFree(ctx->attn_scratch);
+    if (ctx->paged) paged_free(ctx->paged);
     if (ctx->wmem) cudaFree(ctx->wmem);
     if (ctx->smem_pool) cudaFree(ctx->smem_pool);
     delete ctx;
@@ -571,14 +575,14 @@ extern "C" int obs_attn_init(obs_ctx* ctx, const obs_attn_config* ac) {
     const int T = ctx->cfg.max_tokens, H = ctx->sh.H, W = (nq + 2 * nkv) * hd;
     const size_t sizes[] = {(size_t)ac->max_seq * hd * 4, (size_t)T * W * 4, (size_t)T * H * 2, (size_t)T * nq * hd * 2,
                             (size_t)T * nq * hd * 2, (size_t)T * H * 4,
-                            sdpa_part_floats(T, nq, nkv, hd, ctx->num_sms) * 4};
+                            sdpa_part_floats(T, nq, nkv, hd, ctx->num_sms) * 4, (size_t)T * nkv * hd * 4};
     size_t total = 0;
     for (size_t sz : sizes) total += align_up(sz, 256);
     CU(cudaMalloc(&ctx->attn_scratch, total), "attention scratch");
     uint8_t* p = ctx->attn_scratch;
     void** ptrs[] = {(void**)&ctx->rope_cs, (void**)&ctx->a_qkv, (void**)&ctx->a_xn, (void**)&ctx->a_q,
-                     (void**)&ctx->a_out, (void**)&ctx->a_o, (void**)&ctx->a_part};
-    for (int i = 0; i < 7; ++i) *ptrs[i] = p, p += align_up(sizes[i], 256);
+                     (void**)&ctx->a_out, (void**)&ctx->a_o, (void**)&ctx->a_part, (void**)&ctx->a_kv};
+    for (int i = 0; i < 8; ++i) *ptrs[i] = p, p += align_up(sizes[i], 256);
     std::vector<float> tab((size_t)ac->max_seq * hd);
     rope_table(ac->rope_theta, hd, ac->max_seq, tab.data());
     CU(cudaMemcpy(ctx->rope_cs, tab.data(), tab.size() * 4, cudaMemcpyHostToDevice), "rope table");
@@ -662,6 +666,46 @@ extern "C" int obs_attn_forward(obs_ctx* ctx, int layer, const uint16_t* x, uint
     CU(launch_sdpa(ctx->a_q, L.kc, L.vc, T, nq, nkv, hd, ac.max_seq, ac.n_seqs, seq, pos, ctx->a_out, ctx->a_part,
                    ctx->num_sms, st),
        "attention");
+    CU(launch_linear4(L.o_w, L.o_s, L.o_b, ctx->a_out, T, H, nq * hd, ctx->a_o, ctx->num_sms, st), "o projection");
+    CU(launch_residual_add(x, ctx->a_o, (size_t)T * H, out, st), "residual");
+    return OBS_OK;
+}
+
+extern "C" int obs_paged_attn_forward(obs_ctx* ctx, int layer, const obs_paged_kv* kv, const uint16_t* x,
+                                      uint16_t* out, int T, const int32_t* seq, const int32_t* pos,
+                                      const int32_t* slot, const int32_t* q_start, int window, int n_sink,
+                                      float* weights, int w_stride, void* stream) {
+    OBS_CHECK_CTX(ctx);
+    if (ctx->attn.empty()) return fail(ctx, OBS_ERR_STATE, "attention not initialised (obs_attn_init)");
+    if (layer < 0 || layer >= (int)ctx->attn.size()) return fail(ctx, OBS_ERR_INVALID, "layer out of range");
+    if (!ctx->attn[layer].loaded) return fail(ctx, OBS_ERR_STATE, "attention layer not loaded");
+    const auto& ac = ctx->acfg;
+    const auto& L = ctx->attn[layer];
+    const int nq = ac.n_heads, nkv = ac.n_kv_heads, hd = ac.head_dim, H = ctx->sh.H;
+    if (const char* m = paged_mismatch(ctx->paged, nq, nkv, hd))
+        return fail(ctx, ctx->paged ? OBS_ERR_INVALID : OBS_ERR_STATE, m);
+    if (T < 0 || T > ctx->cfg.max_tokens) return fail(ctx, OBS_ERR_INVALID, "T out of range (0..max_tokens)");
+    if (T == 0) return OBS_OK;
+    if (!kv || !x || !out || !seq || !pos || !slot) return fail(ctx, OBS_ERR_INVALID, "null pointer");
+    if (out == x) return fail(ctx, OBS_ERR_INVALID, "out may not alias x");
+    if (!q_start && T != kv->n_seqs) return fail(ctx, OBS_ERR_INVALID, "a decode step (q_start NULL) has one token per sequence");
+    if (q_start && weights) return fail(ctx, OBS_ERR_UNSUPPORTED, "weights are added up by decode steps only");
+    cudaStream_t st = as_stream(stream);
+    uint16_t* krows = ctx->a_kv;
+    uint16_t* vrows = ctx->a_kv + (size_t)ctx->cfg.max_tokens * nkv * hd;
+    CU(launch_rmsnorm(x, L.in_norm, T, H, ctx->cfg.rms_eps, ctx->a_xn, st), "input norm");
+    CU(launch_linear4(L.qkv_w, L.qkv_s, L.qkv_b, ctx->a_xn, T, (nq + 2 * nkv) * hd, H, ctx->a_qkv, ctx->num_sms, st),
+       "qkv projection");
+    CU(launch_qk_norm_rope(ctx->a_qkv, T, nq, nkv, hd, L.q_norm, L.k_norm, ctx->cfg.rms_eps, ctx->rope_cs, ac.max_seq,
+                           seq, pos, ctx->a_q, krows, vrows, kv->n_seqs, ctx->err_flag, st, 1),
+       "q/k norm, rope");
+    int rc = obs_paged_append(ctx, kv, krows, vrows, (int64_t)nkv * hd, seq, slot, T, stream);
+    if (rc == OBS_OK)
+        rc = q_start ? obs_paged_prefill(ctx, kv, ctx->a_q, (int64_t)nq * hd, ctx->a_out, q_start, T, window, n_sink, 0.0f,
+                                         stream)
+                     : obs_paged_decode(ctx, kv, ctx->a_q, (int64_t)nq * hd, ctx->a_out, window, n_sink, 0.0f, weights,
+                                        w_stride, stream);
+    if (rc != OBS_OK) return rc;
     CU(launch_linear4(L.o_w, L.o_s, L.o_b, ctx->a_out, T, H, nq * hd, ctx->a_o, ctx->num_sms, st), "o projection");
     CU(launch_residual_add(x, ctx->a_o, (size_t)T * H, out, st), "residual");
     return OBS_OK;
@@ -1273,6 +1317,8 @@ extern "C" int obs_check_device(obs_ctx* ctx, void* stream) {
                      site[words[2] >= 0 && words[2] <= 6 ? words[2] : 0], words[3]);
             return fail(ctx, OBS_ERR_INVALID, msg);
         }
+        if (flag == kDevBadPage)
+            return fail(ctx, OBS_ERR_INVALID, "device refused a page id outside the pool or a length beyond the table");
         if (flag == kDevBadPos)
             return fail(ctx, OBS_ERR_INVALID, "device refused a token's sequence or position outside the KV caches");
         return fail(ctx, OBS_ERR_INVALID, "device reported an invalid route (expert id out of range)");

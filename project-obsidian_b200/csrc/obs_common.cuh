@@ -20,7 +20,8 @@ constexpr int kBlockBytes = kBlockWords * 4 + 2 * kRowTile * 2;  // + scales + b
 constexpr int kSegAlign = 16;     // expert segments padded to 16 rows (MMA N step)
 
 // Device-side error codes written to the context's flag word.
-enum DevErr : int { kDevOk = 0, kDevTimeout = 1, kDevBadRoute = 2, kDevBadTile = 3, kDevBadSlot = 4, kDevBadPos = 5 };
+enum DevErr : int { kDevOk = 0, kDevTimeout = 1, kDevBadRoute = 2, kDevBadTile = 3, kDevBadSlot = 4, kDevBadPos = 5,
+                    kDevBadPage = 6 };
 // Which check refused a row slot first (word 2 of the flag, next to kDevBadSlot in
 // word 0) and a value it saw (word 3: the slot, row or token it refused).
 enum SlotSite : int {

@@ -221,7 +221,7 @@ cudaError_t launch_linear4(const uint32_t* w, const uint16_t* s, const uint16_t*
 cudaError_t launch_qk_norm_rope(const float* qkv, int T, int nq, int nkv, int hd, const uint16_t* qn,
                                 const uint16_t* kn, float eps, const float* rope_cs, int max_seq, const int32_t* seq,
                                 const int32_t* pos, uint16_t* qout, uint16_t* kcache, uint16_t* vcache, int n_seqs,
-                                int* err, cudaStream_t st);
+                                int* err, cudaStream_t st, int kv_rows = 0);
 // part: sdpa_part_floats(max_tokens, ...) floats of scratch (the splits' partial sums)
 cudaError_t launch_sdpa(const uint16_t* q, const uint16_t* kc, const uint16_t* vc, int T, int nq, int nkv, int hd,
                         int max_seq, int n_seqs, const int32_t* seq, const int32_t* pos, uint16_t* out, float* part,
@@ -231,6 +231,23 @@ size_t sdpa_part_floats(int max_tokens, int nq, int nkv, int hd, int num_sms);
 cudaError_t launch_residual_add(const uint16_t* x, const float* o, size_t n, uint16_t* out, cudaStream_t st);
 // cos/sin of pos * theta^(-2i/hd) for pos < max_seq, i < hd/2, interleaved, computed in double, as fp32
 void rope_table(double theta, int hd, int max_seq, float* out);
+
+// -------------------------------------------------------------- obs_paged.cu
+}  // namespace obs
+struct obs_ctx;
+namespace obs {
+struct PagedState;  // the paged cache's configuration and workspace (obs_paged_init)
+void paged_free(PagedState* p);
+// what obs_paged.cu needs of the context
+struct CtxParts {
+    int device, num_sms;
+    int* err;
+    uint64_t wait_ns;
+    PagedState** paged;
+};
+CtxParts ctx_parts(obs_ctx* ctx);
+// the caller's cache must be the attention block's: heads, KV heads, head_dim, bf16 (else a message)
+const char* paged_mismatch(const PagedState* p, int nq, int nkv, int hd);
 
 // ----------------------------------------------------------------- k_gemm.cu
 enum GemmEpi : int { kEpiSwiglu = 0, kEpiBf16 = 1, kEpiF32 = 2 };

@@ -36,6 +36,8 @@ EXPORTS = (
     "obs_load_layer_safetensors", "obs_expert_file_info", "obs_load_head", "obs_embed", "obs_lm_head",
     "obs_attn_init", "obs_load_attn", "obs_attn_forward", "obs_kv_read", "obs_debug_gemm_tiles",
     "obs_ep_set_placement", "obs_ep_get_placement", "obs_ep_plan_placement",
+    "obs_paged_init", "obs_paged_append", "obs_paged_decode", "obs_paged_prefill", "obs_paged_evict",
+    "obs_paged_attn_forward", "obs_paged_struct_layout",
 )
 EP_HANDLE_BYTES = 64
 STAGES = ("router", "topk", "dispatch", "gemm_gateup", "gemm_down", "combine", "decode_gateup", "decode_down",
@@ -75,6 +77,51 @@ class LayerWeights(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in (
         "router_w", "router_s", "router_b", "gate_w", "gate_s", "gate_b",
         "up_w", "up_s", "up_b", "down_w", "down_s", "down_b")]
+
+
+class PagedConfig(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in (
+        "n_heads", "n_kv_heads", "head_dim", "page_size", "max_seqs", "max_kv_len", "dtype", "weights")]
+
+
+class PagedView(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("block_table", C.c_void_p), ("kv_len", C.c_void_p),
+                ("page_stride", C.c_int64), ("slot_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("n_seqs", C.c_int32), ("n_pages", C.c_int32), ("table_stride", C.c_int32), ("table_pages", C.c_int32)]
+
+
+DTYPE_BF16, DTYPE_F16 = 0, 1
+_DTYPES = {"bf16": DTYPE_BF16, "f16": DTYPE_F16}
+
+
+class PagedKV:
+    """One layer's paged key/value cache (obs_paged_kv) over tensors the caller owns: k and v
+    [n_pages, page_size, n_kv_heads, head_dim] of 16-bit elements (any strides, head_dim
+    consecutive), block_table int32 [n_seqs, pages], kv_len int32 [n_seqs], all on the GPU.
+    Keeps the tensors alive; their contents may change between calls."""
+
+    def __init__(self, k, v, block_table, kv_len):
+        for name, t in (("k", k), ("v", v)):
+            if t.dim() != 4 or t.element_size() != 2 or (t.shape[3] > 1 and t.stride(3) != 1):
+                raise ValueError(f"{name}: [n_pages, page_size, n_kv_heads, head_dim] of 16-bit elements, the last consecutive")
+        if v.shape != k.shape or v.stride() != k.stride() or v.dtype != k.dtype:
+            raise ValueError("k and v must have one shape, one type and the same strides")
+        if block_table.dim() != 2 or block_table.element_size() != 4 or block_table.is_floating_point():
+            raise ValueError("block_table: int32 [n_seqs, pages]")
+        if block_table.shape[1] > 1 and block_table.stride(1) != 1:
+            raise ValueError("block_table's rows must be consecutive")
+        if kv_len.dim() != 1 or kv_len.element_size() != 4 or kv_len.is_floating_point() or not kv_len.is_contiguous():
+            raise ValueError("kv_len: consecutive int32 [n_seqs]")
+        if kv_len.shape[0] != block_table.shape[0]:
+            raise ValueError("kv_len and block_table have different numbers of sequences")
+        if block_table.shape[0] > 1 and block_table.stride(0) < block_table.shape[1]:
+            raise ValueError("block_table's rows may not overlap")
+        self.tensors = (k, v, block_table, kv_len)
+        self.dtype, self.kv_shape = k.dtype, tuple(k.shape[1:])  # kv_shape: page_size, n_kv_heads, head_dim
+        self.view = PagedView(k.data_ptr(), v.data_ptr(), block_table.data_ptr(), kv_len.data_ptr(),
+                              k.stride(0), k.stride(1), k.stride(2), block_table.shape[0], k.shape[0],
+                              block_table.stride(0), block_table.shape[1])
+        self.ref = C.byref(self.view)
 
 
 _LIB = None
@@ -129,6 +176,14 @@ def lib() -> C.CDLL:
         L.obs_load_attn.argtypes = [vp, i32, C.POINTER(AttnWeights), i32]
         L.obs_attn_forward.argtypes = [vp, i32, vp, vp, i32, vp, vp, vp]
         L.obs_kv_read.argtypes = [vp, i32, i32, i32, i32, vp, vp, vp]
+        pp, i64s = C.c_void_p, C.c_int64
+        L.obs_paged_init.argtypes = [vp, C.POINTER(PagedConfig)]
+        L.obs_paged_append.argtypes = [vp, pp, vp, vp, i64s, vp, vp, i32, vp]
+        L.obs_paged_decode.argtypes = [vp, pp, vp, i64s, vp, i32, i32, C.c_float, vp, i32, vp]
+        L.obs_paged_prefill.argtypes = [vp, pp, vp, i64s, vp, vp, i32, i32, i32, C.c_float, vp]
+        L.obs_paged_evict.argtypes = [vp, pp, pp, vp, vp, i32, i32, i32, i32, vp, vp, vp]
+        L.obs_paged_attn_forward.argtypes = [vp, i32, pp, vp, vp, i32, vp, vp, vp, vp, i32, i32, vp, i32, vp]
+        L.obs_paged_struct_layout.argtypes = [C.POINTER(C.c_int32), i32]
         L.obs_set_wait_limit.argtypes = [vp, i64]
         L.obs_probe_wait.argtypes = [vp, vp]
         L.obs_struct_layout.argtypes = [C.POINTER(C.c_int32), i32]
@@ -252,6 +307,91 @@ class MoeContext:
 
     def kv_read(self, layer, seq, pos0, n, k=None, v=None, stream=None):
         self._chk(lib().obs_kv_read(self._h, layer, seq, pos0, n, _ptr(k), _ptr(v), _stream(stream)))
+
+    # -- the paged key/value cache
+    def paged_init(self, n_heads=32, n_kv_heads=4, head_dim=128, page_size=64, max_seqs=1, max_kv_len=4096,
+                   dtype="bf16", weights=False):
+        """The shape of the paged cache and its workspace (once per context); weights: decode steps
+        may add up attention weights."""
+        if dtype not in _DTYPES:
+            raise ValueError(f"dtype must be one of {sorted(_DTYPES)}")
+        pc = PagedConfig(n_heads, n_kv_heads, head_dim, page_size, max_seqs, max_kv_len, _DTYPES[dtype], int(weights))
+        self._chk(lib().obs_paged_init(self._h, C.byref(pc)))
+        self._paged = (page_size, n_kv_heads, head_dim)
+        self._paged_row, self._paged_dtype = n_heads * head_dim, dtype
+
+    def _paged_kv(self, kv):
+        if getattr(self, "_paged", None) is not None:
+            if kv.kv_shape != self._paged:
+                raise ValueError(f"the cache's pages are {kv.kv_shape}, the context's {self._paged}")
+            if ("bf16" if kv.dtype.itemsize == 2 and "bfloat" in str(kv.dtype) else "f16") != self._paged_dtype:
+                raise ValueError(f"the cache holds {kv.dtype}, the context {self._paged_dtype}")
+        return kv.ref
+
+    def _paged_q(self, kv, q, out, rows):
+        """q's row stride, after checks of q and out ([rows, n_heads, head_dim] or [rows, n_heads * head_dim])."""
+        row = self._paged_row
+        if q.dtype != kv.dtype or out.dtype != kv.dtype:
+            raise ValueError(f"q and out must hold {kv.dtype} like the cache")
+        if q.numel() != rows * row or out.numel() != rows * row:
+            raise ValueError(f"q and out must be [{rows}, {row}]")
+        if not out.is_contiguous() or (rows and not q[0].is_contiguous()):
+            raise ValueError("out must be consecutive, and each row of q")
+        return q.stride(0) if rows > 1 else row
+
+    def _paged_w(self, kv, w):
+        if w is None:
+            return None, 0
+        if w.shape[:2] != (kv.view.n_seqs, kv.kv_shape[1]) or w.element_size() != 4 or not w.is_floating_point() \
+                or not w.is_contiguous():
+            raise ValueError("weights: consecutive fp32 [n_seqs, n_kv_heads, positions]")
+        return w.data_ptr(), w.shape[2]
+
+    def paged_append(self, kv, k, v, seq, slot, T, stream=None):
+        """Rows k, v [T, n_kv_heads, head_dim] to positions slot[t] of sequences seq[t]."""
+        ref = self._paged_kv(kv)
+        row = self._paged[1] * self._paged[2]
+        if k.dtype != kv.dtype or v.dtype != kv.dtype or k.numel() < T * row or v.numel() < T * row:
+            raise ValueError(f"k and v must be [T, {row}] of {kv.dtype}")
+        if T and (not k[0].is_contiguous() or not v[0].is_contiguous() or (T > 1 and k.stride(0) != v.stride(0))):
+            raise ValueError("each row of k and v must be consecutive, their strides the same")
+        self._chk(lib().obs_paged_append(self._h, ref, k.data_ptr(), v.data_ptr(), k.stride(0) if T > 1 else row,
+                                         _ptr(seq), _ptr(slot), T, _stream(stream)))
+
+    def paged_decode(self, kv, q, out, window=0, n_sink=0, scale=0.0, weights=None, stream=None):
+        """Attention of each sequence's last position over its pages; weights (optional) += the probabilities."""
+        ref = self._paged_kv(kv)
+        w, ws = self._paged_w(kv, weights)
+        self._chk(lib().obs_paged_decode(self._h, ref, q.data_ptr(), self._paged_q(kv, q, out, kv.view.n_seqs),
+                                         out.data_ptr(), window, n_sink, scale, w, ws, _stream(stream)))
+
+    def paged_prefill(self, kv, q, out, q_start, T, window=0, n_sink=0, scale=0.0, stream=None):
+        """Attention of the sequences' last positions, rows q_start[s] .. q_start[s+1] of q each."""
+        ref = self._paged_kv(kv)
+        self._chk(lib().obs_paged_prefill(self._h, ref, q.data_ptr(), self._paged_q(kv, q, out, T), out.data_ptr(),
+                                          _ptr(q_start), T, window, n_sink, scale, _stream(stream)))
+
+    def paged_evict(self, kv, dst, weights, weights_dst, budget, n_sink=0, n_recent=0, kept=None, new_len=None,
+                    stream=None):
+        """Keeps `budget` positions per sequence and KV head, moved to dst; kept int32 [n_seqs,
+        n_kv_heads, budget] and new_len int32 [n_seqs] are written."""
+        ref, to = self._paged_kv(kv), self._paged_kv(dst)
+        w, ws = self._paged_w(kv, weights)
+        wd, wds = self._paged_w(kv, weights_dst)
+        if wd is not None and wds != ws:
+            raise ValueError("weights and weights_dst must have one shape")
+        if kept is not None and kept.numel() < kv.view.n_seqs * kv.kv_shape[1] * budget:
+            raise ValueError("kept: int32 [n_seqs, n_kv_heads, budget]")
+        self._chk(lib().obs_paged_evict(self._h, ref, to, w, wd, ws, budget, n_sink, n_recent, _ptr(kept),
+                                        _ptr(new_len), _stream(stream)))
+
+    def paged_attn_forward(self, layer, kv, x, out, T, seq, pos, slot, q_start=None, window=0, n_sink=0, weights=None,
+                           stream=None):
+        """attn_forward over a paged cache: a decode step (q_start None) or prompts' new tokens."""
+        w, ws = self._paged_w(kv, weights)
+        self._chk(lib().obs_paged_attn_forward(self._h, layer, self._paged_kv(kv), _ptr(x), _ptr(out), T, _ptr(seq),
+                                               _ptr(pos), _ptr(slot), _ptr(q_start), window, n_sink, w, ws,
+                                               _stream(stream)))
 
     def synth_layer(self, layer: int, seed: int = 0):
         self._chk(lib().obs_synth_layer(self._h, layer, seed))
@@ -394,6 +534,14 @@ def plan_placement(load, world: int) -> list:
     if rc != 0:
         raise ObsError(rc, "obs_ep_plan_placement: bad arguments")
     return list(out)
+
+
+def paged_struct_layout() -> list[int]:
+    """sizeof and field offsets of obs_paged_config and obs_paged_kv, as the library was compiled."""
+    n = lib().obs_paged_struct_layout(None, 0)
+    buf = (C.c_int32 * n)()
+    lib().obs_paged_struct_layout(buf, n)
+    return list(buf)
 
 
 def struct_layout() -> list[int]:
