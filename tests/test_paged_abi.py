@@ -5,10 +5,12 @@ import ctypes as C
 import pytest
 
 import obsmoe
+import test_abi
 from test_abi import header_struct_fields, rust_struct_layout
 
 
-def test_paged_struct_layout_of_library_ctypes_and_rust_agree():
+def test_paged_struct_layout_of_library_ctypes_and_rust_agree(monkeypatch):
+    monkeypatch.setitem(test_abi.RUST_TYPES, "i64", (8, 8))
     v = obsmoe.paged_struct_layout()
     assert len(v) == 21
     at = 0
