@@ -15,6 +15,10 @@ int ctx_fail(obs_ctx* ctx, int code, const char* msg);  // obs_api.cu
 struct PagedState {
     obs_paged_config cfg{};
     uint8_t* mem = nullptr;
+    float* part = nullptr;      // parts of items that several CTAs share
+    uint32_t* count = nullptr;  // their arrivals
+    float* scores = nullptr;    // with cfg.weights: [max_seqs][n_heads][max_kv_len]
+    float2* ml = nullptr;       // with cfg.weights: [max_seqs][n_heads]
 };
 
 void paged_free(PagedState* p) {
@@ -35,6 +39,8 @@ const char* paged_mismatch(const PagedState* p, int nq, int nkv, int hd) {
 using namespace obs;
 
 namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -109,6 +115,28 @@ extern "C" int obs_paged_init(obs_ctx* ctx, const obs_paged_config* cfg) {
     PagedState* ps = new (std::nothrow) PagedState();
     if (!ps) return ctx_fail(ctx, OBS_ERR_NOMEM, "paged cache state");
     ps->cfg = *cfg;
+    const size_t n = (size_t)cfg->max_seqs * nq;
+    const size_t sizes[] = {paged_decode_part_floats(nq / nkv, parts.num_sms) * 4, (size_t)kPagedCtas * parts.num_sms * 4,
+                            cfg->weights ? n * cfg->max_kv_len * 4 : 0, cfg->weights ? n * 8 : 0};
+    void** ptrs[] = {(void**)&ps->part, (void**)&ps->count, (void**)&ps->scores, (void**)&ps->ml};
+    size_t total = 0;
+    for (size_t sz : sizes) total += (sz + 255) / 256 * 256;
+    cudaError_t e = cudaSetDevice(parts.device);
+    if (e == cudaSuccess) e = cudaMalloc(&ps->mem, total);
+    if (e != cudaSuccess) {
+        cudaGetLastError();  // the failed allocation is reported here, not by a later call
+        delete ps;
+        return ctx_fail(ctx, e == cudaErrorMemoryAllocation ? OBS_ERR_NOMEM : OBS_ERR_CUDA,
+                        (std::string("paged workspace: ") + cudaGetErrorString(e)).c_str());
+    }
+    uint8_t* at = ps->mem;
+    for (int i = 0; i < 4; ++i) *ptrs[i] = sizes[i] ? at : nullptr, at += (sizes[i] + 255) / 256 * 256;
+    e = cudaMemset(ps->count, 0, sizes[1]);
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();  // the calls may come on any stream
+    if (e != cudaSuccess) {
+        paged_free(ps);
+        return ctx_fail(ctx, OBS_ERR_CUDA, (std::string("paged workspace: ") + cudaGetErrorString(e)).c_str());
+    }
     *parts.paged = ps;
     return OBS_OK;
 }
@@ -135,11 +163,13 @@ extern "C" int obs_paged_decode(obs_ctx* ctx, const obs_paged_kv* kv, const void
     if (const char* m = query_args(a, q, q_stride, out, window, n_sink, scale)) return ctx_fail(ctx, OBS_ERR_INVALID, m);
     if (weights && !ps->cfg.weights)
         return ctx_fail(ctx, OBS_ERR_STATE, "the paged cache was initialised without room for weights");
-    if (weights && w_stride < a.cap && w_stride <= 0) return ctx_fail(ctx, OBS_ERR_INVALID, "w_stride must be positive");
+    if (weights && w_stride <= 0) return ctx_fail(ctx, OBS_ERR_INVALID, "w_stride must be positive");
     if (weights && w_stride < a.cap) a.cap = w_stride;  // a longer sequence is refused on the device
-    AttnRowsArgs p{a, reinterpret_cast<const uint16_t*>(q), q_stride, reinterpret_cast<uint16_t*>(out), nullptr,
-                   0, window, n_sink, scale > 0.0f ? scale : 1.0f / sqrtf((float)a.hd), weights, w_stride};
-    return launched(ctx, launch_paged_attn_rows(p, ps->cfg.dtype, as_stream(stream)), "paged decode");
+    const float sc = scale > 0.0f ? scale : 1.0f / sqrtf((float)a.hd);
+    DecodeArgs p{a, reinterpret_cast<const uint16_t*>(q), q_stride, reinterpret_cast<uint16_t*>(out), window, n_sink,
+                 sc * kLog2e, ps->part, ps->count, weights ? ps->scores : nullptr, ps->cfg.max_kv_len,
+                 weights ? ps->ml : nullptr, weights, w_stride};
+    return launched(ctx, launch_paged_decode(p, ps->cfg.dtype, parts.num_sms, as_stream(stream)), "paged decode");
 }
 
 extern "C" int obs_paged_prefill(obs_ctx* ctx, const obs_paged_kv* kv, const void* q, int64_t q_stride, void* out,

@@ -98,6 +98,24 @@ struct AttnRowsArgs {
     float* weights;           // decode, optional: [n_seqs][nkv][w_stride]
     int w_stride;
 };
+constexpr int kPagedCtas = 2;  // CTAs per SM of the decode kernel
+struct DecodeArgs {
+    PagedArgs c;
+    const uint16_t* q;        // [n_seqs][nq][hd], rows q_stride elements apart
+    int64_t q_stride;
+    uint16_t* out;            // [n_seqs][nq][hd]
+    int window, n_sink;
+    float scale_log2;         // scale * log2(e)
+    float* part;              // 2 per CTA: its parts of (sequence, head)s it shares
+    uint32_t* count;          // [CTAs] arrivals, zero between launches
+    float* scores;            // with weights: [n_seqs][nq][score_ld] x_j
+    int64_t score_ld;
+    float2* ml;               // with weights: [n_seqs][nq] maximum and sum
+    float* weights;           // optional: [n_seqs][nkv][w_stride]
+    int w_stride;
+};
+cudaError_t launch_paged_decode(const DecodeArgs& p, int dtype, int num_sms, cudaStream_t st);
+size_t paged_decode_part_floats(int group, int num_sms);
 cudaError_t launch_paged_append(const PagedArgs& a, const uint16_t* k, const uint16_t* v, int64_t row_stride,
                                 const int32_t* seq, const int32_t* slot, int T, int num_sms, cudaStream_t st);
 cudaError_t launch_paged_evict(const PagedArgs& src, const PagedArgs& dst, const float* w, float* w_dst, int w_stride,
