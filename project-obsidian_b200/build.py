@@ -20,7 +20,7 @@ OUT = os.path.join(HERE, "libobsmoe.so")
 BUILD = os.path.join(HERE, "_build")
 SOURCES = ["obs_api.cu", "obs_static.cu", "obs_safetensors.cu", "k_synth.cu", "k_router.cu", "k_dispatch.cu",
            "k_decode.cu", "k_gemm.cu", "k_ep.cu", "k_head.cu", "k_attn.cu", "obs_paged.cu", "k_paged.cu",
-           "k_paged_decode.cu"]
+           "k_paged_decode.cu", "k_paged_prefill.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -1,0 +1,609 @@
+// k_paged_prefill.cu -- causal attention of prompts (or chunks of them) over their
+// pages, with a sliding window and a few first positions that stay visible, on
+// tcgen05.
+//
+//   out[t][h] = sum_j p_j v_j,  p = softmax over the visible j of scale * q[t][h] . k_j
+//
+// Rows: the query heads of one KV head and the new tokens of one sequence are one
+// line of rows, row R = token * group + head of the group, so the heads share the
+// tiles of K and V and a block of 256 rows spans only 256 / group tokens: few tiles
+// lie across the causal diagonal or the window's edge, and a chunk of a few tokens
+// still fills the tensor cores' 128 rows.
+//
+// One CTA takes one block of 256 rows, two tiles of 128 (A and B), against the
+// 128-position tiles that any of them sees (sinks, then the window):
+//   S = Q . K^T     128 x 128 fp32 in TMEM; Q and K in shared memory, K-major
+//   P = 2^(S scale log2 e - m)   in registers, one row per thread, written back over
+//                   S as 16-bit values, the A operand of
+//   O += P . V      128 x head_dim fp32 in TMEM; V as it lies (its rows are the
+//                   reduction: the N-major form of the B operand)
+// Sixteen warps:
+//   0-3, 4-7   softmax of tile A, of tile B: running maximum m and sum l of the
+//              thread's row.  O is rescaled only when the maximum has grown by more
+//              than 2^8 (p stays below 2^8, far inside both types), by the same
+//              threads, between a tile's S and its P, when no product touches O
+//   8          issues the products: PV_A, QK_A of the next tile, PV_B, QK_B, ..., so
+//              one tile's softmax runs under the other's products
+//   12-15      loads: rows of K and V by page, 16 bytes per cp.async, into the
+//              128-byte-swizzled tiles (rows that no query of the block sees as zeros)
+// What bounds it: for head_dim 128 the exponentials (16 a clock and SM) take as long
+// as the products (8192 operations a clock).
+//
+// p is rounded to 16 bits once; over many positions the roundings average out far
+// below the output's own.  Where a row of the block sees fewer than kFewKeys
+// positions they do not, and what the rounding left is multiplied too (the other
+// half of S's columns holds it): half as much work again for the first tiles of a
+// prompt.
+//
+// A NaN or infinity in V meets p = 0 of rows that do not see it, and 0 * NaN is NaN:
+// a row whose result is not finite is computed again from its visible positions
+// alone (attend_row).  When nothing is wrong this costs a comparison.
+//
+// Few rows, long axis: where there are fewer blocks than SMs the tiles of a block
+// are split over several CTAs, whose (m, l, O) k_paged_join puts together in order.
+// Every wait is bounded as in k_gemm.cu.
+#include "paged.cuh"
+
+namespace obs {
+namespace {
+
+constexpr int kRows = 256, kKeys = 128;
+constexpr int kFewKeys = 512;
+constexpr int kThreads = 512;
+constexpr int kWarpMma = 8, kWarpLd = 12, kLdWarps = 4;
+constexpr float kRescale = 8.0f;  // log2 of the growth of the maximum that O tolerates
+
+template <int HD>
+struct Pf {
+    static constexpr int HALF = kKeys * 128;          // 128 rows x 64 elements, swizzled
+    static constexpr int TILE = (HD / 64) * HALF;
+    static constexpr int NST = HD == 128 ? 4 : 8;     // K and V stages
+    static constexpr int RING = 2 * TILE;             // after Q's two tiles
+    static constexpr int BAR = RING + NST * TILE;
+    static constexpr int NBAR = 2 * NST + 1 + 2 * 4 + 1;
+    static constexpr int SMEM = BAR + NBAR * 8 + 1024;
+    static constexpr int O = 256;                     // TMEM column of O_A; O_B at + 128; S at 0, 128
+};
+
+enum Wait : int { kWtEmpty = 31, kWtFull, kWtQ, kWtS, kWtP, kWtPv, kWtO };
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+// 32 lanes x 32 consecutive fp32 columns (no wait)
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Instruction descriptor, kind::f16: fp32 sums, both operands of one 16-bit type;
+// bnk: B is N-major (its rows are the reduction).
+template <int DT>
+__device__ __forceinline__ uint32_t idesc16(int M, int N, bool bnk) {
+    const uint32_t f = DT == 0 ? 1u : 0u;  // bf16 : f16
+    return (1u << 4) | (f << 7) | (f << 10) | (bnk ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+// N-major operand, 128-byte swizzle: 64 elements of N side by side in a row, 8 rows
+// of the reduction per 1 KB; `next` bytes to the following 64 elements of N.
+__device__ __forceinline__ uint64_t sw128_desc_n(uint32_t saddr, uint32_t next) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr & 0x3FFFF) >> 4);
+    d |= (uint64_t)(next >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+
+// The tiles that a block of rows at positions i_lo .. i_hi sees.
+struct Tiles {
+    int ts, wt, nt;        // sink tiles, the window's first tile, tiles in all
+    int lo, hi, sink_end;  // positions some row sees: j < sink_end or lo <= j < hi
+};
+__device__ __forceinline__ Tiles tiles_of(int i_lo, int i_hi, int window, int n_sink) {
+    Tiles t;
+    t.hi = max(i_hi + 1, 0);
+    t.lo = min(window_lo(max(i_lo, 0), window), t.hi);
+    t.sink_end = min(n_sink, t.lo);
+    t.ts = (t.sink_end + kKeys - 1) / kKeys;
+    t.wt = max(t.ts, t.lo / kKeys);
+    t.nt = t.ts + max(0, (t.hi + kKeys - 1) / kKeys - t.wt);
+    return t;
+}
+// positions the query at i sees
+__device__ __forceinline__ int seen(int i, int window, int n_sink) {
+    const int lo = window_lo(i, window);
+    return i + 1 - lo + min(n_sink, lo);
+}
+
+// The row of q (and out) that line row R of (sequence, KV head) stands for.
+__device__ __forceinline__ int64_t row_of(const PagedArgs& a, int q0, int h, int R, int* token) {
+    const int t = R / a.group, g = R - t * a.group;
+    *token = q0 + t;
+    return h * a.group + g;
+}
+
+template <int DT>
+__device__ __forceinline__ void recompute_row(const PrefillArgs& p, int s, int h, int64_t t, int head, int i) {
+    using X = Elem<DT>;
+    const PagedArgs& a = p.c;
+    const int lane = threadIdx.x & 31;
+    const uint16_t* q = p.q + t * p.q_stride + head * a.hd;
+    float qf[4] = {0.0f, 0.0f, 0.0f, 0.0f}, acc[4], m, l;
+    if (4 * lane < a.hd) {
+        const uint2 w = *reinterpret_cast<const uint2*>(q + 4 * lane);
+        qf[0] = X::lo(w.x), qf[1] = X::hi(w.x), qf[2] = X::lo(w.y), qf[3] = X::hi(w.y);
+    }
+    const int lo = window_lo(i, p.window);
+    attend_row<DT>(a, s, h, qf, p.scale, min(p.n_sink, lo), lo, i + 1, acc, m, l);
+    if (4 * lane < a.hd)
+        *reinterpret_cast<uint2*>(p.out + (t * a.nkv * a.group + head) * a.hd + 4 * lane) =
+            make_uint2(X::pack(acc[0] / l, acc[1] / l), X::pack(acc[2] / l, acc[3] / l));
+}
+
+template <int DT, int HD>
+__global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
+    pdl_begin();
+    using X = Elem<DT>;
+    using C = Pf<HD>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ int s_scan[kThreads / 32], s_total;
+    __shared__ int s_seq, s_blk;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort;
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t sbase = smem_u32(smem), bars = sbase + C::BAR;
+    auto full = [&](int s) { return bars + 8 * s; };
+    auto empty = [&](int s) { return bars + 8 * (C::NST + s); };
+    const uint32_t qfull = bars + 8 * (2 * C::NST);
+    auto sfull = [&](int x) { return qfull + 8 + 8 * x; };
+    auto pfull = [&](int x) { return qfull + 24 + 8 * x; };
+    auto pvdone = [&](int x) { return qfull + 40 + 8 * x; };
+    auto ofull = [&](int x) { return qfull + 56 + 8 * x; };
+    const uint32_t mma_done = qfull + 72;
+    const PagedArgs& a = p.c;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    volatile int* abort = &s_abort;
+
+    // ---- which block of rows: blocks of all the sequences in one line, the last
+    // (the longest of their sequence) first; the KV heads of a block side by side
+    const int h = blockIdx.x % a.nkv, bi = blockIdx.x / a.nkv, z = blockIdx.y;
+    {
+        const int per = (a.n_seqs + kThreads - 1) / kThreads;
+        const int sb = min(a.n_seqs, tid * per), se = min(a.n_seqs, sb + per);
+        int mine = 0;
+        bool bad = tid == 0 && (p.q_start[0] != 0 || p.q_start[a.n_seqs] != p.T);
+        for (int s = sb; s < se; ++s) {
+            const int q0 = p.q_start[s], q1 = p.q_start[s + 1];
+            if (q0 < 0 || q1 < q0 || q1 > p.T) bad = true;
+            else mine += ((q1 - q0) * a.group + kRows - 1) / kRows;
+        }
+        if (bad) atomicExch(a.err, kDevBadPos);
+        int incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        if (lane == 31) s_scan[warp] = incl;
+        if (tid == 0) s_seq = -1;
+        __syncthreads();
+        int before = incl - mine, total = 0;
+#pragma unroll
+        for (int w = 0; w < kThreads / 32; ++w) {
+            if (w < warp) before += s_scan[w];
+            total += s_scan[w];
+        }
+        const int want = total - 1 - bi;
+        int b = before;
+        for (int s = sb; s < se; ++s) {
+            const int q0 = p.q_start[s], q1 = p.q_start[s + 1];
+            if (q0 < 0 || q1 < q0 || q1 > p.T) continue;
+            const int c = ((q1 - q0) * a.group + kRows - 1) / kRows;
+            if (want >= b && want < b + c) s_seq = s, s_blk = want - b;
+            b += c;
+        }
+        __syncthreads();
+    }
+    const int s = s_seq;
+    if (s < 0) return;
+    const int q0 = p.q_start[s], nrow = (p.q_start[s + 1] - q0) * a.group;
+    const int R0 = s_blk * kRows, rows = min(kRows, nrow - R0);
+    const bool hasB = rows > kKeys;
+    const int base = seq_len(a, s) - (p.q_start[s + 1] - q0);  // position of the sequence's first new token
+    const int i_lo = base + R0 / a.group, i_hi = base + (R0 + rows - 1) / a.group;
+    const Tiles tl = tiles_of(i_lo, i_hi, p.window, p.n_sink);
+    const bool split = p.splits > 1;
+    const int ns = min(p.splits, tl.nt);
+    const int nq = a.nkv * a.group;
+    if (z >= ns) {  // nothing (or nothing more) to see
+        for (int r = tid; r < rows; r += kThreads) {
+            int t;
+            const int64_t head = row_of(a, q0, h, R0 + r, &t);
+            if (split) p.part_ml[((int64_t)z * p.T + t) * nq + head] = make_float2(-INFINITY, 0.0f);
+            else
+                for (int d = 0; d < a.hd; d += 8)
+                    *reinterpret_cast<uint4*>(p.out + ((int64_t)t * nq + head) * a.hd + d) = make_uint4(0, 0, 0, 0);
+        }
+        return;
+    }
+    const int x0 = (int)((int64_t)tl.nt * z / ns), x1 = (int)((int64_t)tl.nt * (z + 1) / ns), nt = x1 - x0;
+    auto tile_key = [&](int x) { return (x < tl.ts ? x : x - tl.ts + tl.wt) * kKeys; };
+    const bool precise = i_lo < 0 || seen(i_lo, p.window, p.n_sink) < kFewKeys;
+
+    if (tid == 0) {
+        for (int i = 0; i < C::NST; ++i) mbar_init(full(i), kLdWarps), mbar_init(empty(i), 1);
+        mbar_init(qfull, kLdWarps);
+        for (int x = 0; x < 2; ++x) mbar_init(sfull(x), 1), mbar_init(pfull(x), 4), mbar_init(pvdone(x), 1), mbar_init(ofull(x), 1);
+        mbar_init(mma_done, 1);
+        s_abort = 0;
+        fence_mbar_init();
+    }
+    if (warp == kWarpMma) {
+        tmem_alloc(smem_u32(&s_tmem), 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+
+    if (warp >= kWarpLd) {
+        // ------------------------------------------------------------- loads
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        const int w = warp - kWarpLd;
+        constexpr int CH = HD / 8, RPI = 32 / CH;       // pieces per row, rows per instruction
+        constexpr int NI = kKeys / (kLdWarps * RPI);    // instructions per tile and warp
+        const int ch = lane % CH, rsub = lane / CH, chunks = a.hd / 8;
+        // piece ch of row r of a tile: half ch / 8, row r, piece (ch % 8) ^ (r % 8)
+        auto place = [&](int r) { return (uint32_t)((ch >> 3) * C::HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4)); };
+        for (int x = 0; x < (hasB ? 2 : 1); ++x)
+#pragma unroll 4
+            for (int i = 0; i < NI; ++i) {
+                const int r = (i * kLdWarps + w) * RPI + rsub, R = R0 + x * kKeys + r;
+                const bool take = x * kKeys + r < rows && ch < chunks;
+                int t = 0;
+                const int64_t head = take ? row_of(a, q0, h, R, &t) : 0;
+                cp16(sbase + x * C::TILE + place(r), p.q + (take ? t * p.q_stride + head * a.hd + ch * 8 : 0), take);
+            }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        // each lane looks up NI * RPI / 32 rows of the warp's share: lane l those of i = l / RPI + 32 / RPI * k
+        constexpr int NL = NI * RPI / 32;
+        static_assert(NL >= 1 && NI * RPI % 32 == 0, "one lookup or more per lane");
+        int64_t off[NL];
+        auto lookup = [&](int x) {
+            const int k0 = tile_key(x);
+#pragma unroll
+            for (int k = 0; k < NL; ++k) {
+                const int i = lane / RPI + k * (32 / RPI);
+                const int j = k0 + (i * kLdWarps + w) * RPI + lane % RPI;
+                off[k] = j < tl.sink_end || (j >= tl.lo && j < tl.hi) ? row_offset(a, s, j, h) : -1;
+            }
+        };
+        lookup(x0);
+        bool ok = true;
+        for (int n = 0; n < 2 * nt && ok; ++n) {
+            const int st = n % C::NST;
+            if (!__all_sync(0xffffffffu, mbar_wait(empty(st), ((n / C::NST) & 1) ^ 1, abort, kWtEmpty, p.wait_ns))) {
+                ok = false;
+                break;
+            }
+            const uint16_t* pool = (n & 1) ? a.v : a.k;
+            const uint32_t dst = sbase + C::RING + st * C::TILE;
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int r = (i * kLdWarps + w) * RPI + rsub;
+                const int64_t o = __shfl_sync(0xffffffffu, off[i / (32 / RPI)], (i % (32 / RPI)) * RPI + rsub);
+                const bool take = o >= 0 && ch < chunks;
+                cp16(dst + place(r), pool + (take ? o + ch * 8 : 0), take);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if ((n & 1) && n + 1 < 2 * nt) lookup(x0 + (n + 1) / 2);
+            // the load before this one has landed: hand it to the tensor cores
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(n ? full((n - 1) % C::NST) : qfull);
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (ok && lane == 0) mbar_arrive(full((2 * nt - 1) % C::NST));
+    } else if (warp >= kWarpMma) {
+        // ---------------------------------------------------------- products
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == kWarpMma) {
+            const uint32_t id_qk = idesc16<DT>(128, kKeys, false), id_pv = idesc16<DT>(128, HD, true);
+            const int nx = hasB ? 2 : 1;
+            auto wait = [&](uint32_t bar, int par, int code) {
+                return __all_sync(0xffffffffu, mbar_wait(bar, par & 1, abort, code, p.wait_ns));
+            };
+            auto qk = [&](int x, int st) {
+                const uint64_t qd = sw128_desc(sbase + x * C::TILE), kd = sw128_desc(sbase + C::RING + st * C::TILE);
+#pragma unroll
+                for (int kk = 0; kk < HD / 16; ++kk) {
+                    const uint64_t step = (uint64_t)((kk >> 2) * (C::HALF >> 4) + 2 * (kk & 3));
+                    tc_mma_f16(tmem + x * kKeys, qd + step, kd + step, id_qk, kk != 0);
+                }
+                tc_commit(sfull(x));
+            };
+            auto pv = [&](int x, int st, bool first) {
+                const uint64_t vd = sw128_desc_n(sbase + C::RING + st * C::TILE, C::HALF);
+                const uint32_t o = tmem + C::O + x * 128;
+#pragma unroll
+                for (int kk = 0; kk < kKeys / 16; ++kk)
+                    tc_mma_f16_ts(o, tmem + x * kKeys + kk * 8, vd + kk * (2048 >> 4), id_pv, !(first && kk == 0));
+                if (precise) {
+#pragma unroll
+                    for (int kk = 0; kk < kKeys / 16; ++kk)
+                        tc_mma_f16_ts(o, tmem + x * kKeys + 64 + kk * 8, vd + kk * (2048 >> 4), id_pv, 1);
+                }
+            };
+            bool ok = wait(qfull, 0, kWtQ) && wait(full(0), 0, kWtFull);
+            tc_fence_after();
+            if (ok && elect_one()) {
+                for (int x = 0; x < nx; ++x) qk(x, 0);
+                tc_commit(empty(0));
+            }
+            __syncwarp();
+            for (int j = 0; j < nt && ok; ++j) {
+                const int vn = 2 * j + 1, vs = vn % C::NST, kn = vn + 1, ks = kn % C::NST;
+                ok = wait(full(vs), vn / C::NST, kWtFull);
+                const bool more = j + 1 < nt;
+                for (int x = 0; x < nx && ok; ++x) {
+                    ok = wait(pfull(x), j, kWtP);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        pv(x, vs, j == 0);
+                        tc_commit(more ? pvdone(x) : ofull(x));
+                        if (x == nx - 1) tc_commit(empty(vs));
+                    }
+                    __syncwarp();
+                    if (!more) continue;
+                    // S of the next tile takes P's columns: the product that reads them must be done
+                    ok = (x > 0 || wait(full(ks), kn / C::NST, kWtFull)) && wait(pvdone(x), j, kWtPv);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        qk(x, ks);
+                        if (x == nx - 1) tc_commit(empty(ks));
+                    }
+                    __syncwarp();
+                }
+            }
+            // every product has finished before the CTA frees its tensor memory, also when a role gave up
+            if (elect_one()) tc_commit(mma_done);
+            __syncwarp();
+            const uint64_t t0 = global_ns();
+            while (!mbar_try_wait(mma_done, 0) && global_ns() - t0 < p.wait_ns) {
+            }
+        }
+    } else if (warp < 4 || hasB) {
+        // ----------------------------------------------------------- softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+        const int x = warp >> 2, r = x * kKeys + (warp & 3) * 32 + lane;
+        const uint32_t tq = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t ts = tq + x * kKeys, to = tq + C::O + x * 128;
+        const bool valid = r < rows;
+        int t;
+        const int64_t head = row_of(a, q0, h, R0 + min(r, rows - 1), &t);
+        const int i = base + (t - q0), lo = window_lo(i, p.window);
+        int i_min = i, lo_max = lo;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            i_min = min(i_min, __shfl_xor_sync(0xffffffffu, i_min, o));
+            lo_max = max(lo_max, __shfl_xor_sync(0xffffffffu, lo_max, o));
+        }
+        float m = -INFINITY, l = 0.0f;
+        bool ok = true;
+        for (int j = 0; j < nt; ++j) {
+            if (!__all_sync(0xffffffffu, mbar_wait(sfull(x), j & 1, abort, kWtS, p.wait_ns))) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            float v[kKeys];
+#pragma unroll
+            for (int c = 0; c < kKeys; c += 32) tmem_ld32(ts + c, v + c);
+            tc_wait_ld();
+            const int k0 = tile_key(x0 + j);
+            if (!(k0 + kKeys - 1 <= i_min && (k0 >= lo_max || k0 + kKeys <= p.n_sink))) {
+#pragma unroll
+                for (int c = 0; c < kKeys; ++c) {
+                    const int k = k0 + c;
+                    if (k > i || (k < lo && k >= p.n_sink)) v[c] = -INFINITY;
+                }
+            }
+            float mx[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+            for (int c = 4; c < kKeys; ++c) mx[c & 3] = fmaxf(mx[c & 3], v[c]);
+            const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2);
+            if (__any_sync(0xffffffffu, mn > m + kRescale)) {
+                const float corr = mn == -INFINITY ? 1.0f : ex2(m - mn);
+                m = mn;
+                l *= corr;
+                if (j > 0) {
+#pragma unroll
+                    for (int c = 0; c < HD; c += 32) {
+                        float o[32];
+                        tmem_ld32(to + c, o);
+                        tc_wait_ld();
+                        uint32_t w[32];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * corr);
+                        tmem_st32(to + c, w);
+                    }
+                }
+            }
+            const float ref = m == -INFINITY ? 0.0f : m;
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c0 = 0; c0 < kKeys; c0 += 64) {
+                uint32_t w[32];
+#pragma unroll
+                for (int c = 0; c < 64; c += 2) {
+                    const float a0 = ex2(fmaf(v[c0 + c], p.scale_log2, -ref));
+                    const float a1 = ex2(fmaf(v[c0 + c + 1], p.scale_log2, -ref));
+                    v[c0 + c] = a0, v[c0 + c + 1] = a1;
+                    sum[c & 2] += a0, sum[(c & 2) + 1] += a1;
+                    w[c / 2] = X::pack(a0, a1);
+                }
+                tmem_st32(ts + c0 / 2, w);
+                if (precise) {
+#pragma unroll
+                    for (int c = 0; c < 64; c += 2)
+                        w[c / 2] = X::pack(v[c0 + c] - X::lo(w[c / 2]), v[c0 + c + 1] - X::hi(w[c / 2]));
+                    tmem_st32(ts + 64 + c0 / 2, w);
+                }
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(pfull(x));
+        }
+        // ------------------------------------------------------- the rows out
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(ofull(x), 0, abort, kWtO, p.wait_ns));
+        if (ok) {
+            tc_fence_after();
+            const int64_t row = (int64_t)t * nq + head;
+            bool bad = false;
+            if (split && valid) p.part_ml[(int64_t)z * p.T * nq + row] = make_float2(m, l);
+#pragma unroll
+            for (int c = 0; c < HD; c += 32) {
+                float o[32];
+                tmem_ld32(to + c, o);
+                tc_wait_ld();
+                if (split) {
+                    float4* dst = reinterpret_cast<float4*>(p.part_acc + ((int64_t)z * p.T * nq + row) * HD + c);
+                    if (valid)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                } else {
+                    const float inv = 1.0f / l;
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        float y[8];
+#pragma unroll
+                        for (int b = 0; b < 8; ++b) {
+                            y[b] = i < 0 ? 0.0f : o[e + b] * inv;
+                            bad |= !(fabsf(y[b]) <= 3.4e38f);
+                        }
+                        if (valid && c + e < a.hd)
+                            *reinterpret_cast<uint4*>(p.out + row * a.hd + c + e) =
+                                make_uint4(X::pack(y[0], y[1]), X::pack(y[2], y[3]), X::pack(y[4], y[5]), X::pack(y[6], y[7]));
+                    }
+                }
+            }
+            uint32_t again = __ballot_sync(0xffffffffu, bad && valid);
+            while (again) {  // (never with split: k_paged_join does it)
+                const int who = __ffs(again) - 1;
+                again &= again - 1;
+                recompute_row<DT>(p, s, h, __shfl_sync(0xffffffffu, t, who), __shfl_sync(0xffffffffu, (int)head, who),
+                                  __shfl_sync(0xffffffffu, i, who));
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == kWarpMma) tmem_dealloc(tmem, 512);
+    if (tid == 0 && s_abort) {
+        atomicExch(a.err + 1, s_abort);
+        atomicExch(a.err, kDevTimeout);
+    }
+}
+
+// The splits' parts of each row, in their order: one warp per (token, query head).
+template <int DT, int HD>
+__global__ void __launch_bounds__(256) k_paged_join(PrefillArgs p) {
+    pdl_begin();
+    using X = Elem<DT>;
+    const PagedArgs& a = p.c;
+    const int lane = threadIdx.x & 31, nq = a.nkv * a.group;
+    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= (int64_t)p.T * nq) return;
+    const int t = (int)(row / nq), head = (int)(row - (int64_t)t * nq);
+    int s, i;
+    if (!find_row(a, p.q_start, t, p.T, &s, &i)) return;
+    const int64_t step = (int64_t)p.T * nq;
+    float mx = -INFINITY;
+    for (int z = 0; z < p.splits; ++z) mx = fmaxf(mx, p.part_ml[z * step + row].x);
+    const float ref = mx == -INFINITY ? 0.0f : mx;
+    constexpr int PER = HD / 32;
+    float o[PER] = {}, l = 0.0f;
+#pragma unroll 4
+    for (int z = 0; z < p.splits; ++z) {
+        const float2 ml = p.part_ml[z * step + row];
+        if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // an unused split, or one that saw only -inf
+        const float f = ex2(ml.x - ref);
+        l += f * ml.y;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) o[e] += f * p.part_acc[(z * step + row) * HD + e * 32 + lane];
+    }
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        const int d = e * 32 + lane;
+        const float y = i < 0 ? 0.0f : o[e] / l;
+        bad |= !(fabsf(y) <= 3.4e38f);
+        if (d < a.hd) p.out[row * a.hd + d] = X::h(y);
+    }
+    if (__any_sync(0xffffffffu, bad)) recompute_row<DT>(p, s, head / a.group, t, head, i);
+}
+
+template <int DT, int HD>
+cudaError_t launch_t(const PrefillArgs& p, int blocks, cudaStream_t st) {
+    constexpr int smem = Pf<HD>::SMEM;
+    static_assert(smem <= 232448 - 1024, "smem");
+    auto kern = k_paged_prefill<DT, HD>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    e = launch_pdl(kern, dim3(blocks, p.splits), dim3(kThreads), smem, st, p);
+    if (e == cudaSuccess && p.splits > 1)
+        e = launch_pdl(k_paged_join<DT, HD>, dim3((unsigned)(((int64_t)p.T * p.c.nkv * p.c.group + 7) / 8)), dim3(256), 0, st, p);
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+}  // namespace
+
+// (blocks of a call that splits) * splits <= num_sms, 256 rows each
+size_t paged_prefill_part_floats(int num_sms) { return (size_t)num_sms * kRows * (128 + 2); }
+
+cudaError_t launch_paged_prefill(PrefillArgs p, float* part, int dtype, int num_sms, cudaStream_t st) {
+    const PagedArgs& a = p.c;
+    if (p.T <= 0 || a.n_seqs <= 0) return cudaSuccess;
+    if (a.hd > 128 || a.hd % 8 || a.group > kPagedMaxGroup) return cudaErrorInvalidValue;
+    // at most this many blocks of rows: every sequence's last one may be ragged
+    const int64_t blocks = ((int64_t)p.T * a.group / kRows + (a.n_seqs < p.T ? a.n_seqs : p.T)) * a.nkv;
+    if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
+    int splits = (int)(num_sms / blocks);
+    const int most = (a.cap + 2 * kKeys - 1) / (2 * kKeys);  // two tiles or more each
+    if (splits > most) splits = most;
+    p.splits = splits < 1 ? 1 : splits;
+    const int64_t rows = (int64_t)p.T * a.nkv * a.group * p.splits;
+    p.part_acc = part;
+    p.part_ml = reinterpret_cast<float2*>(part + rows * (a.hd > 64 ? 128 : 64));
+    const int b = (int)blocks;
+    if (dtype) return a.hd > 64 ? launch_t<1, 128>(p, b, st) : launch_t<1, 64>(p, b, st);
+    return a.hd > 64 ? launch_t<0, 128>(p, b, st) : launch_t<0, 64>(p, b, st);
+}
+
+}  // namespace obs

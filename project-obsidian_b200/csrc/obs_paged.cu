@@ -18,6 +18,7 @@ struct PagedState {
     float* part = nullptr;      // parts of items that several CTAs share
     uint32_t* count = nullptr;  // their arrivals
     float* scores = nullptr;    // with cfg.weights: [max_seqs][n_heads][max_kv_len]
+    float* pf_part = nullptr;   // parts of a prefill's rows that several CTAs share
     float2* ml = nullptr;       // with cfg.weights: [max_seqs][n_heads]
 };
 
@@ -117,8 +118,9 @@ extern "C" int obs_paged_init(obs_ctx* ctx, const obs_paged_config* cfg) {
     ps->cfg = *cfg;
     const size_t n = (size_t)cfg->max_seqs * nq;
     const size_t sizes[] = {paged_decode_part_floats(nq / nkv, parts.num_sms) * 4, (size_t)kPagedCtas * parts.num_sms * 4,
-                            cfg->weights ? n * cfg->max_kv_len * 4 : 0, cfg->weights ? n * 8 : 0};
-    void** ptrs[] = {(void**)&ps->part, (void**)&ps->count, (void**)&ps->scores, (void**)&ps->ml};
+                            cfg->weights ? n * cfg->max_kv_len * 4 : 0, cfg->weights ? n * 8 : 0,
+                            paged_prefill_part_floats(parts.num_sms) * 4};
+    void** ptrs[] = {(void**)&ps->part, (void**)&ps->count, (void**)&ps->scores, (void**)&ps->ml, (void**)&ps->pf_part};
     size_t total = 0;
     for (size_t sz : sizes) total += (sz + 255) / 256 * 256;
     cudaError_t e = cudaSetDevice(parts.device);
@@ -130,7 +132,7 @@ extern "C" int obs_paged_init(obs_ctx* ctx, const obs_paged_config* cfg) {
                         (std::string("paged workspace: ") + cudaGetErrorString(e)).c_str());
     }
     uint8_t* at = ps->mem;
-    for (int i = 0; i < 4; ++i) *ptrs[i] = sizes[i] ? at : nullptr, at += (sizes[i] + 255) / 256 * 256;
+    for (int i = 0; i < 5; ++i) *ptrs[i] = sizes[i] ? at : nullptr, at += (sizes[i] + 255) / 256 * 256;
     e = cudaMemset(ps->count, 0, sizes[1]);
     if (e == cudaSuccess) e = cudaDeviceSynchronize();  // the calls may come on any stream
     if (e != cudaSuccess) {
@@ -180,9 +182,11 @@ extern "C" int obs_paged_prefill(obs_ctx* ctx, const obs_paged_kv* kv, const voi
     if (a.n_seqs == 0) return ctx_fail(ctx, OBS_ERR_INVALID, "rows without sequences");
     if (!q_start) return ctx_fail(ctx, OBS_ERR_INVALID, "null pointer");
     if (const char* m = query_args(a, q, q_stride, out, window, n_sink, scale)) return ctx_fail(ctx, OBS_ERR_INVALID, m);
-    AttnRowsArgs p{a, reinterpret_cast<const uint16_t*>(q), q_stride, reinterpret_cast<uint16_t*>(out), q_start,
-                   T, window, n_sink, scale > 0.0f ? scale : 1.0f / sqrtf((float)a.hd), nullptr, 0};
-    return launched(ctx, launch_paged_attn_rows(p, ps->cfg.dtype, as_stream(stream)), "paged prefill");
+    const float sc = scale > 0.0f ? scale : 1.0f / sqrtf((float)a.hd);
+    PrefillArgs p{a, reinterpret_cast<const uint16_t*>(q), q_stride, reinterpret_cast<uint16_t*>(out), q_start, T, window,
+                  n_sink, sc, sc * kLog2e, parts.wait_ns, 1, nullptr, nullptr};
+    return launched(ctx, launch_paged_prefill(p, ps->pf_part, ps->cfg.dtype, parts.num_sms, as_stream(stream)),
+                    "paged prefill");
 }
 
 extern "C" int obs_paged_evict(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_kv* dst, const float* weights,

@@ -116,6 +116,23 @@ struct DecodeArgs {
 };
 cudaError_t launch_paged_decode(const DecodeArgs& p, int dtype, int num_sms, cudaStream_t st);
 size_t paged_decode_part_floats(int group, int num_sms);
+struct PrefillArgs {
+    PagedArgs c;
+    const uint16_t* q;        // [T][nq][hd], rows q_stride elements apart
+    int64_t q_stride;
+    uint16_t* out;            // [T][nq][hd]
+    const int32_t* q_start;   // [n_seqs + 1]
+    int T;
+    int window, n_sink;
+    float scale, scale_log2;  // scale_log2 = scale * log2(e)
+    uint64_t wait_ns;
+    // set by the launcher
+    int splits;
+    float* part_acc;          // [splits][T][nq][64 or 128]
+    float2* part_ml;          // [splits][T][nq]
+};
+cudaError_t launch_paged_prefill(PrefillArgs p, float* part, int dtype, int num_sms, cudaStream_t st);
+size_t paged_prefill_part_floats(int num_sms);
 cudaError_t launch_paged_append(const PagedArgs& a, const uint16_t* k, const uint16_t* v, int64_t row_stride,
                                 const int32_t* seq, const int32_t* slot, int T, int num_sms, cudaStream_t st);
 cudaError_t launch_paged_evict(const PagedArgs& src, const PagedArgs& dst, const float* w, float* w_dst, int w_stride,
