@@ -60,17 +60,51 @@ struct Pf {
     static constexpr int NST = HD == 128 ? 4 : 8;     // K and V stages
     static constexpr int RING = 2 * TILE;             // after Q's two tiles
     static constexpr int BAR = RING + NST * TILE;
-    static constexpr int NBAR = 2 * NST + 1 + 2 * 4 + 1;
+    static constexpr int NBAR = 2 * NST + 1 + 2 * 5 + 1;
     static constexpr int SMEM = BAR + NBAR * 8 + 1024;
     static constexpr int O = 256;                     // TMEM column of O_A; O_B at + 128; S at 0, 128
 };
 
 enum Wait : int { kWtEmpty = 31, kWtFull, kWtQ, kWtS, kWtP, kWtPv, kWtO };
 
+// mbar_wait without the suspend hint (waits here are shorter than waking up takes)
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile int* abort, int code,
+                                         uint64_t limit_ns) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = global_ns();
+    for (;;) {
+#pragma unroll 1
+        for (int i = 0; i < 64; ++i)
+            if (mbar_try_wait(bar, parity)) return true;
+        if (*abort) return false;
+        if (global_ns() - t0 > limit_ns) {
+            *abort = code;
+            return false;
+        }
+    }
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// two at once: (a0, a1) * s + c
+__device__ __forceinline__ void fma2(float& a0, float& a1, float s, float c) {
+    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %2};\n\tmov.b64 c, {%3, %3};\n\t"
+        "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "+f"(a0), "+f"(a1)
+        : "f"(s), "f"(c));
+}
+__device__ __forceinline__ void add2(float& s0, float& s1, float a0, float a1) {
+    asm("{\n\t.reg .b64 s, a;\n\tmov.b64 s, {%0, %1};\n\tmov.b64 a, {%2, %3};\n\tadd.rn.f32x2 s, s, a;\n\t"
+        "mov.b64 {%0, %1}, s;\n\t}"
+        : "+f"(s0), "+f"(s1)
+        : "f"(a0), "f"(a1));
 }
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
@@ -130,9 +164,15 @@ __device__ __forceinline__ int seen(int i, int window, int n_sink) {
     return i + 1 - lo + min(n_sink, lo);
 }
 
-// The row of q (and out) that line row R of (sequence, KV head) stands for.
-__device__ __forceinline__ int64_t row_of(const PagedArgs& a, int q0, int h, int R, int* token) {
-    const int t = R / a.group, g = R - t * a.group;
+// the n lowest bits set (none for n <= 0, all from 32)
+__device__ __forceinline__ uint32_t low_bits(int n) {
+    return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+}
+
+// The row of q (and out) that line row R of (sequence, KV head) stands for.  R / group
+// as in page_of: R < 2^20 * 16 <= 2^32 / group.
+__device__ __forceinline__ int row_of(const PagedArgs& a, uint32_t magic, int q0, int h, int R, int* token) {
+    const int t = magic ? (int)__umulhi((uint32_t)R, magic) : R, g = R - t * a.group;
     *token = q0 + t;
     return h * a.group + g;
 }
@@ -161,8 +201,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
     using X = Elem<DT>;
     using C = Pf<HD>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ int s_scan[kThreads / 32], s_total;
-    __shared__ int s_seq, s_blk;
+    __shared__ int s_scan[kThreads / 32];
+    __shared__ int s_blk[5];  // sequence, block of it, its rows' range, its length
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -171,10 +211,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
     auto empty = [&](int s) { return bars + 8 * (C::NST + s); };
     const uint32_t qfull = bars + 8 * (2 * C::NST);
     auto sfull = [&](int x) { return qfull + 8 + 8 * x; };
-    auto pfull = [&](int x) { return qfull + 24 + 8 * x; };
-    auto pvdone = [&](int x) { return qfull + 40 + 8 * x; };
-    auto ofull = [&](int x) { return qfull + 56 + 8 * x; };
-    const uint32_t mma_done = qfull + 72;
+    auto pfull = [&](int x) { return qfull + 24 + 8 * x; };  // of the first 64 positions; of the others at + 16
+    auto pvdone = [&](int x) { return qfull + 56 + 8 * x; };
+    auto ofull = [&](int x) { return qfull + 72 + 8 * x; };
+    const uint32_t mma_done = qfull + 88;
     const PagedArgs& a = p.c;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     volatile int* abort = &s_abort;
@@ -185,12 +225,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
     {
         const int per = (a.n_seqs + kThreads - 1) / kThreads;
         const int sb = min(a.n_seqs, tid * per), se = min(a.n_seqs, sb + per);
-        int mine = 0;
+        int mine = 0, len0 = 0, q0 = 0, q1 = 0;  // of the thread's first sequence, at hand when it is the block's
         bool bad = tid == 0 && (p.q_start[0] != 0 || p.q_start[a.n_seqs] != p.T);
         for (int s = sb; s < se; ++s) {
-            const int q0 = p.q_start[s], q1 = p.q_start[s + 1];
-            if (q0 < 0 || q1 < q0 || q1 > p.T) bad = true;
-            else mine += ((q1 - q0) * a.group + kRows - 1) / kRows;
+            const int b0 = p.q_start[s], b1 = p.q_start[s + 1];
+            if (s == sb) len0 = seq_len(a, s), q0 = b0, q1 = b1;
+            if (b0 < 0 || b1 < b0 || b1 > p.T) bad = true;
+            else mine += ((b1 - b0) * a.group + kRows - 1) / kRows;
         }
         if (bad) atomicExch(a.err, kDevBadPos);
         int incl = mine;
@@ -200,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
             if (lane >= o) incl += y;
         }
         if (lane == 31) s_scan[warp] = incl;
-        if (tid == 0) s_seq = -1;
+        if (tid == 0) s_blk[0] = -1;
         __syncthreads();
         int before = incl - mine, total = 0;
 #pragma unroll
@@ -209,22 +250,28 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
             total += s_scan[w];
         }
         const int want = total - 1 - bi;
-        int b = before;
-        for (int s = sb; s < se; ++s) {
-            const int q0 = p.q_start[s], q1 = p.q_start[s + 1];
-            if (q0 < 0 || q1 < q0 || q1 > p.T) continue;
-            const int c = ((q1 - q0) * a.group + kRows - 1) / kRows;
-            if (want >= b && want < b + c) s_seq = s, s_blk = want - b;
-            b += c;
+        if (want >= before && want < before + mine) {
+            int b = before;
+            for (int s = sb; s < se; ++s) {
+                if (s > sb) q0 = p.q_start[s], q1 = p.q_start[s + 1];
+                if (q0 < 0 || q1 < q0 || q1 > p.T) continue;
+                const int c = ((q1 - q0) * a.group + kRows - 1) / kRows;
+                if (want < b + c) {
+                    s_blk[0] = s, s_blk[1] = want - b, s_blk[2] = q0, s_blk[3] = q1;
+                    s_blk[4] = s == sb ? len0 : seq_len(a, s);
+                    break;
+                }
+                b += c;
+            }
         }
         __syncthreads();
     }
-    const int s = s_seq;
+    const int s = s_blk[0];
     if (s < 0) return;
-    const int q0 = p.q_start[s], nrow = (p.q_start[s + 1] - q0) * a.group;
-    const int R0 = s_blk * kRows, rows = min(kRows, nrow - R0);
+    const int q0 = s_blk[2], nrow = (s_blk[3] - q0) * a.group;
+    const int R0 = s_blk[1] * kRows, rows = min(kRows, nrow - R0);
     const bool hasB = rows > kKeys;
-    const int base = seq_len(a, s) - (p.q_start[s + 1] - q0);  // position of the sequence's first new token
+    const int base = s_blk[4] - (s_blk[3] - q0);  // position of the sequence's first new token
     const int i_lo = base + R0 / a.group, i_hi = base + (R0 + rows - 1) / a.group;
     const Tiles tl = tiles_of(i_lo, i_hi, p.window, p.n_sink);
     const bool split = p.splits > 1;
@@ -233,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
     if (z >= ns) {  // nothing (or nothing more) to see
         for (int r = tid; r < rows; r += kThreads) {
             int t;
-            const int64_t head = row_of(a, q0, h, R0 + r, &t);
+            const int head = row_of(a, p.group_magic, q0, h, R0 + r, &t);
             if (split) p.part_ml[((int64_t)z * p.T + t) * nq + head] = make_float2(-INFINITY, 0.0f);
             else
                 for (int d = 0; d < a.hd; d += 8)
@@ -247,8 +294,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
 
     if (tid == 0) {
         for (int i = 0; i < C::NST; ++i) mbar_init(full(i), kLdWarps), mbar_init(empty(i), 1);
-        mbar_init(qfull, kLdWarps);
-        for (int x = 0; x < 2; ++x) mbar_init(sfull(x), 1), mbar_init(pfull(x), 4), mbar_init(pvdone(x), 1), mbar_init(ofull(x), 1);
+        mbar_init(qfull, hasB ? 8 : 4);
+        for (int x = 0; x < 2; ++x) mbar_init(sfull(x), 1), mbar_init(pfull(x), 4), mbar_init(pfull(x) + 16, 4), mbar_init(pvdone(x), 1), mbar_init(ofull(x), 1);
         mbar_init(mma_done, 1);
         s_abort = 0;
         fence_mbar_init();
@@ -271,16 +318,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
         const int ch = lane % CH, rsub = lane / CH, chunks = a.hd / 8;
         // piece ch of row r of a tile: half ch / 8, row r, piece (ch % 8) ^ (r % 8)
         auto place = [&](int r) { return (uint32_t)((ch >> 3) * C::HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4)); };
-        for (int x = 0; x < (hasB ? 2 : 1); ++x)
-#pragma unroll 4
-            for (int i = 0; i < NI; ++i) {
-                const int r = (i * kLdWarps + w) * RPI + rsub, R = R0 + x * kKeys + r;
-                const bool take = x * kKeys + r < rows && ch < chunks;
-                int t = 0;
-                const int64_t head = take ? row_of(a, q0, h, R, &t) : 0;
-                cp16(sbase + x * C::TILE + place(r), p.q + (take ? t * p.q_stride + head * a.hd + ch * 8 : 0), take);
-            }
-        asm volatile("cp.async.commit_group;" ::: "memory");
         // each lane looks up NI * RPI / 32 rows of the warp's share: lane l those of i = l / RPI + 32 / RPI * k
         constexpr int NL = NI * RPI / 32;
         static_assert(NL >= 1 && NI * RPI % 32 == 0, "one lookup or more per lane");
@@ -298,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
         bool ok = true;
         for (int n = 0; n < 2 * nt && ok; ++n) {
             const int st = n % C::NST;
-            if (!__all_sync(0xffffffffu, mbar_wait(empty(st), ((n / C::NST) & 1) ^ 1, abort, kWtEmpty, p.wait_ns))) {
+            if (!__all_sync(0xffffffffu, wait_bar(empty(st), ((n / C::NST) & 1) ^ 1, abort, kWtEmpty, p.wait_ns))) {
                 ok = false;
                 break;
             }
@@ -314,10 +351,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
             asm volatile("cp.async.commit_group;" ::: "memory");
             if ((n & 1) && n + 1 < 2 * nt) lookup(x0 + (n + 1) / 2);
             // the load before this one has landed: hand it to the tensor cores
+            if (n == 0) continue;
             asm volatile("cp.async.wait_group 1;" ::: "memory");
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(n ? full((n - 1) % C::NST) : qfull);
+            if (lane == 0) mbar_arrive(full((n - 1) % C::NST));
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         fence_proxy_async_smem();
@@ -330,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
             const uint32_t id_qk = idesc16<DT>(128, kKeys, false), id_pv = idesc16<DT>(128, HD, true);
             const int nx = hasB ? 2 : 1;
             auto wait = [&](uint32_t bar, int par, int code) {
-                return __all_sync(0xffffffffu, mbar_wait(bar, par & 1, abort, code, p.wait_ns));
+                return __all_sync(0xffffffffu, wait_bar(bar, par & 1, abort, code, p.wait_ns));
             };
             auto qk = [&](int x, int st) {
                 const uint64_t qd = sw128_desc(sbase + x * C::TILE), kd = sw128_desc(sbase + C::RING + st * C::TILE);
@@ -341,16 +379,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
                 }
                 tc_commit(sfull(x));
             };
-            auto pv = [&](int x, int st, bool first) {
+            auto pv = [&](int x, int st, int half, bool first) {
                 const uint64_t vd = sw128_desc_n(sbase + C::RING + st * C::TILE, C::HALF);
                 const uint32_t o = tmem + C::O + x * 128;
 #pragma unroll
-                for (int kk = 0; kk < kKeys / 16; ++kk)
-                    tc_mma_f16_ts(o, tmem + x * kKeys + kk * 8, vd + kk * (2048 >> 4), id_pv, !(first && kk == 0));
+                for (int i = 0; i < kKeys / 32; ++i) {
+                    const int kk = half * (kKeys / 32) + i;
+                    tc_mma_f16_ts(o, tmem + x * kKeys + kk * 8, vd + kk * (2048 >> 4), id_pv, !(first && i == 0));
+                }
                 if (precise) {
 #pragma unroll
-                    for (int kk = 0; kk < kKeys / 16; ++kk)
+                    for (int i = 0; i < kKeys / 32; ++i) {
+                        const int kk = half * (kKeys / 32) + i;
                         tc_mma_f16_ts(o, tmem + x * kKeys + 64 + kk * 8, vd + kk * (2048 >> 4), id_pv, 1);
+                    }
                 }
             };
             bool ok = wait(qfull, 0, kWtQ) && wait(full(0), 0, kWtFull);
@@ -368,8 +410,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
                     ok = wait(pfull(x), j, kWtP);
                     if (!ok) break;
                     tc_fence_after();
+                    if (elect_one()) pv(x, vs, 0, j == 0);
+                    __syncwarp();
+                    ok = wait(pfull(x) + 16, j, kWtP);
+                    if (!ok) break;
+                    tc_fence_after();
                     if (elect_one()) {
-                        pv(x, vs, j == 0);
+                        pv(x, vs, 1, false);
                         tc_commit(more ? pvdone(x) : ofull(x));
                         if (x == nx - 1) tc_commit(empty(vs));
                     }
@@ -400,8 +447,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
         const uint32_t tq = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t ts = tq + x * kKeys, to = tq + C::O + x * 128;
         const bool valid = r < rows;
+        {
+            // the warp's 32 rows of Q: piece ch of row r lies in half ch / 8 at (ch % 8) ^ (r % 8)
+            constexpr int CH = HD / 8, RPI = 32 / CH;
+            const int ch = lane % CH, r0 = x * kKeys + (warp & 3) * 32 + lane / CH;
+            const bool in = ch < a.hd / 8;
+#pragma unroll 8
+            for (int k = 0; k < CH; ++k) {
+                const int rr = r0 + k * RPI, rt = rr - x * kKeys;
+                const bool take = in && rr < rows;
+                int tt = 0;
+                const int hh = take ? row_of(a, p.group_magic, q0, h, R0 + rr, &tt) : 0;
+                cp16(sbase + x * C::TILE + (ch >> 3) * C::HALF + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4),
+                     p.q + (take ? tt * p.q_stride + (int64_t)hh * a.hd + ch * 8 : 0), take);
+            }
+            asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(qfull);
+        }
         int t;
-        const int64_t head = row_of(a, q0, h, R0 + min(r, rows - 1), &t);
+        const int head = row_of(a, p.group_magic, q0, h, R0 + min(r, rows - 1), &t);
         const int i = base + (t - q0), lo = window_lo(i, p.window);
         int i_min = i, lo_max = lo;
 #pragma unroll
@@ -409,10 +475,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
             i_min = min(i_min, __shfl_xor_sync(0xffffffffu, i_min, o));
             lo_max = max(lo_max, __shfl_xor_sync(0xffffffffu, lo_max, o));
         }
-        float m = -INFINITY, l = 0.0f;
+        float m0 = -INFINITY, m = -INFINITY, l = 0.0f;  // running maximum of q . k; the one in use, scaled
         bool ok = true;
         for (int j = 0; j < nt; ++j) {
-            if (!__all_sync(0xffffffffu, mbar_wait(sfull(x), j & 1, abort, kWtS, p.wait_ns))) {
+            if (!__all_sync(0xffffffffu, wait_bar(sfull(x), j & 1, abort, kWtS, p.wait_ns))) {
                 ok = false;
                 break;
             }
@@ -423,30 +489,34 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
             tc_wait_ld();
             const int k0 = tile_key(x0 + j);
             if (!(k0 + kKeys - 1 <= i_min && (k0 >= lo_max || k0 + kKeys <= p.n_sink))) {
+                // bit c of word w: column 32 w + c is visible (below i + 1, and a sink or in the window)
 #pragma unroll
-                for (int c = 0; c < kKeys; ++c) {
-                    const int k = k0 + c;
-                    if (k > i || (k < lo && k >= p.n_sink)) v[c] = -INFINITY;
+                for (int w = 0; w < kKeys / 32; ++w) {
+                    const int b = k0 + 32 * w;
+                    const uint32_t vis = low_bits(i + 1 - b) & (~low_bits(lo - b) | low_bits(p.n_sink - b));
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) v[32 * w + c] = (vis >> c) & 1u ? v[32 * w + c] : -INFINITY;
                 }
             }
-            float mx[4] = {v[0], v[1], v[2], v[3]};
+            float mx[4] = {m0, v[0], v[1], v[2]};
 #pragma unroll
-            for (int c = 4; c < kKeys; ++c) mx[c & 3] = fmaxf(mx[c & 3], v[c]);
-            const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2);
+            for (int c = 3; c + 1 < kKeys; c += 2) mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], v[c], v[c + 1]);
+            m0 = max3(fmaxf(mx[0], v[kKeys - 1]), mx[1], fmaxf(mx[2], mx[3]));
+            const float mn = m0 * p.scale_log2;
             if (__any_sync(0xffffffffu, mn > m + kRescale)) {
                 const float corr = mn == -INFINITY ? 1.0f : ex2(m - mn);
                 m = mn;
                 l *= corr;
                 if (j > 0) {
 #pragma unroll
-                    for (int c = 0; c < HD; c += 32) {
-                        float o[32];
-                        tmem_ld32(to + c, o);
+                    for (int c = 0; c < HD; c += 16) {
+                        float o[16];
+                        tmem_ld16(to + c, o);
                         tc_wait_ld();
-                        uint32_t w[32];
+                        uint32_t w[16];
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * corr);
-                        tmem_st32(to + c, w);
+                        for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(o[e] * corr);
+                        tmem_st16(to + c, w);
                     }
                 }
             }
@@ -457,10 +527,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
                 uint32_t w[32];
 #pragma unroll
                 for (int c = 0; c < 64; c += 2) {
-                    const float a0 = ex2(fmaf(v[c0 + c], p.scale_log2, -ref));
-                    const float a1 = ex2(fmaf(v[c0 + c + 1], p.scale_log2, -ref));
-                    v[c0 + c] = a0, v[c0 + c + 1] = a1;
-                    sum[c & 2] += a0, sum[(c & 2) + 1] += a1;
+                    float &a0 = v[c0 + c], &a1 = v[c0 + c + 1];
+                    fma2(a0, a1, p.scale_log2, -ref);
+                    a0 = ex2(a0), a1 = ex2(a1);
+                    add2(sum[c & 2], sum[(c & 2) + 1], a0, a1);
                     w[c / 2] = X::pack(a0, a1);
                 }
                 tmem_st32(ts + c0 / 2, w);
@@ -470,51 +540,50 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
                         w[c / 2] = X::pack(v[c0 + c] - X::lo(w[c / 2]), v[c0 + c + 1] - X::hi(w[c / 2]));
                     tmem_st32(ts + 64 + c0 / 2, w);
                 }
+                // half of the positions: their products may start
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(pfull(x) + (c0 ? 16 : 0));
             }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tc_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(pfull(x));
         }
         // ------------------------------------------------------- the rows out
-        ok = ok && __all_sync(0xffffffffu, mbar_wait(ofull(x), 0, abort, kWtO, p.wait_ns));
+        ok = ok && __all_sync(0xffffffffu, wait_bar(ofull(x), 0, abort, kWtO, p.wait_ns));
         if (ok) {
             tc_fence_after();
             const int64_t row = (int64_t)t * nq + head;
             bool bad = false;
             if (split && valid) p.part_ml[(int64_t)z * p.T * nq + row] = make_float2(m, l);
+            float o[HD];
 #pragma unroll
-            for (int c = 0; c < HD; c += 32) {
-                float o[32];
-                tmem_ld32(to + c, o);
-                tc_wait_ld();
-                if (split) {
-                    float4* dst = reinterpret_cast<float4*>(p.part_acc + ((int64_t)z * p.T * nq + row) * HD + c);
-                    if (valid)
+            for (int c = 0; c < HD; c += 32) tmem_ld32(to + c, o + c);
+            tc_wait_ld();
+            if (split) {
+                float4* dst = reinterpret_cast<float4*>(p.part_acc + ((int64_t)z * p.T * nq + row) * HD);
+                if (valid)
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-                } else {
-                    const float inv = 1.0f / l;
+                    for (int e = 0; e < HD / 4; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            } else {
+                const float inv = i < 0 ? 0.0f : 1.0f / l;
 #pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
-                        float y[8];
+                for (int e = 0; e < HD; e += 8) {
+                    float y[8];
 #pragma unroll
-                        for (int b = 0; b < 8; ++b) {
-                            y[b] = i < 0 ? 0.0f : o[e + b] * inv;
-                            bad |= !(fabsf(y[b]) <= 3.4e38f);
-                        }
-                        if (valid && c + e < a.hd)
-                            *reinterpret_cast<uint4*>(p.out + row * a.hd + c + e) =
-                                make_uint4(X::pack(y[0], y[1]), X::pack(y[2], y[3]), X::pack(y[4], y[5]), X::pack(y[6], y[7]));
+                    for (int b = 0; b < 8; ++b) {
+                        y[b] = i < 0 ? 0.0f : o[e + b] * inv;
+                        bad |= !(fabsf(y[b]) <= 3.4e38f);
                     }
+                    if (valid && e < a.hd)
+                        *reinterpret_cast<uint4*>(p.out + row * a.hd + e) =
+                            make_uint4(X::pack(y[0], y[1]), X::pack(y[2], y[3]), X::pack(y[4], y[5]), X::pack(y[6], y[7]));
                 }
             }
             uint32_t again = __ballot_sync(0xffffffffu, bad && valid);
             while (again) {  // (never with split: k_paged_join does it)
                 const int who = __ffs(again) - 1;
                 again &= again - 1;
-                recompute_row<DT>(p, s, h, __shfl_sync(0xffffffffu, t, who), __shfl_sync(0xffffffffu, (int)head, who),
+                recompute_row<DT>(p, s, h, __shfl_sync(0xffffffffu, t, who), __shfl_sync(0xffffffffu, head, who),
                                   __shfl_sync(0xffffffffu, i, who));
             }
         }
@@ -598,6 +667,7 @@ cudaError_t launch_paged_prefill(PrefillArgs p, float* part, int dtype, int num_
     const int most = (a.cap + 2 * kKeys - 1) / (2 * kKeys);  // two tiles or more each
     if (splits > most) splits = most;
     p.splits = splits < 1 ? 1 : splits;
+    p.group_magic = a.group == 1 ? 0u : (uint32_t)((1ull << 32) / (uint32_t)a.group + 1);
     const int64_t rows = (int64_t)p.T * a.nkv * a.group * p.splits;
     p.part_acc = part;
     p.part_ml = reinterpret_cast<float2*>(part + rows * (a.hd > 64 ? 128 : 64));

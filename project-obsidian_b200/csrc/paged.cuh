@@ -130,6 +130,7 @@ struct PrefillArgs {
     int splits;
     float* part_acc;          // [splits][T][nq][64 or 128]
     float2* part_ml;          // [splits][T][nq]
+    uint32_t group_magic;     // for row_of
 };
 cudaError_t launch_paged_prefill(PrefillArgs p, float* part, int dtype, int num_sms, cudaStream_t st);
 size_t paged_prefill_part_floats(int num_sms);
