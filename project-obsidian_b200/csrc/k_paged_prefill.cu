@@ -22,10 +22,13 @@
 //              thread's row.  O is rescaled only when the maximum has grown by more
 //              than 2^8 (p stays below 2^8, far inside both types), by the same
 //              threads, between a tile's S and its P, when no product touches O
-//   8          issues the products: PV_A, QK_A of the next tile, PV_B, QK_B, ..., so
-//              one tile's softmax runs under the other's products
+//   8, 9       issue the products of tile A, of tile B: PV of a tile of positions, then
+//              QK of the tile after the next into the columns that this P leaves
 //   12-15      loads: rows of K and V by page, 16 bytes per cp.async, into the
-//              128-byte-swizzled tiles (rows that no query of the block sees as zeros)
+//              128-byte-swizzled tiles (rows that no query of the block sees as zeros);
+//              a stage's barrier counts the pieces as they land, and the fence that lets
+//              the tensor cores see them is the issuing warp's (in the loading warps it
+//              would wait for every load in flight)
 // What bounds it: for head_dim 128 the exponentials (16 a clock and SM) take as long
 // as the products (8192 operations a clock).
 //
@@ -47,7 +50,7 @@
 namespace obs {
 namespace {
 
-constexpr int kRows = 256, kKeys = 128;
+constexpr int kRows = 256, kM = 128, kKeys = 64;
 constexpr int kFewKeys = 512;
 constexpr int kThreads = 512;
 constexpr int kWarpMma = 8, kWarpLd = 12, kLdWarps = 4;
@@ -55,14 +58,16 @@ constexpr float kRescale = 8.0f;  // log2 of the growth of the maximum that O to
 
 template <int HD>
 struct Pf {
-    static constexpr int HALF = kKeys * 128;          // 128 rows x 64 elements, swizzled
-    static constexpr int TILE = (HD / 64) * HALF;
-    static constexpr int NST = HD == 128 ? 4 : 8;     // K and V stages
-    static constexpr int RING = 2 * TILE;             // after Q's two tiles
-    static constexpr int BAR = RING + NST * TILE;
-    static constexpr int NBAR = 2 * NST + 1 + 2 * 5 + 1;
+    static constexpr int NH = HD / 64;                // 64-element halves of a row
+    static constexpr int QHALF = kM * 128, QTILE = NH * QHALF;    // rows x 128 bytes, swizzled
+    static constexpr int HALF = kKeys * 128, TILE = NH * HALF;
+    static constexpr int STAGE = 2 * TILE;            // K of tiles 0 and 1, then V of tile j with K of tile j + 2
+    static constexpr int NST = HD == 128 ? 4 : 8;
+    static constexpr int RING = 2 * QTILE;
+    static constexpr int BAR = RING + NST * STAGE;
+    static constexpr int NBAR = 2 * NST + 1 + 2 * 7 + 1;
     static constexpr int SMEM = BAR + NBAR * 8 + 1024;
-    static constexpr int O = 256;                     // TMEM column of O_A; O_B at + 128; S at 0, 128
+    static constexpr int O = 256;                     // TMEM: S of tile x, buffer b at 128 x + 64 b; O at 256 + 128 x
 };
 
 enum Wait : int { kWtEmpty = 31, kWtFull, kWtQ, kWtS, kWtP, kWtPv, kWtO };
@@ -210,11 +215,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
     auto full = [&](int s) { return bars + 8 * s; };
     auto empty = [&](int s) { return bars + 8 * (C::NST + s); };
     const uint32_t qfull = bars + 8 * (2 * C::NST);
-    auto sfull = [&](int x) { return qfull + 8 + 8 * x; };
-    auto pfull = [&](int x) { return qfull + 24 + 8 * x; };  // of the first 64 positions; of the others at + 16
-    auto pvdone = [&](int x) { return qfull + 56 + 8 * x; };
-    auto ofull = [&](int x) { return qfull + 72 + 8 * x; };
-    const uint32_t mma_done = qfull + 88;
+    auto sfull = [&](int x, int b) { return qfull + 8 + 8 * (2 * x + b); };
+    auto pfull = [&](int x, int b) { return qfull + 40 + 8 * (2 * x + b); };
+    auto pvdone = [&](int x, int b) { return qfull + 72 + 8 * (2 * x + b); };
+    auto ofull = [&](int x) { return qfull + 104 + 8 * x; };
+    const uint32_t mma_done = qfull + 120;
     const PagedArgs& a = p.c;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     volatile int* abort = &s_abort;
@@ -270,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
     if (s < 0) return;
     const int q0 = s_blk[2], nrow = (s_blk[3] - q0) * a.group;
     const int R0 = s_blk[1] * kRows, rows = min(kRows, nrow - R0);
-    const bool hasB = rows > kKeys;
+    const bool hasB = rows > kM;
     const int base = s_blk[4] - (s_blk[3] - q0);  // position of the sequence's first new token
     const int i_lo = base + R0 / a.group, i_hi = base + (R0 + rows - 1) / a.group;
     const Tiles tl = tiles_of(i_lo, i_hi, p.window, p.n_sink);
@@ -293,10 +298,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
     const bool precise = i_lo < 0 || seen(i_lo, p.window, p.n_sink) < kFewKeys;
 
     if (tid == 0) {
-        for (int i = 0; i < C::NST; ++i) mbar_init(full(i), kLdWarps), mbar_init(empty(i), 1);
+        for (int i = 0; i < C::NST; ++i) mbar_init(full(i), 32 * kLdWarps), mbar_init(empty(i), hasB ? 2 : 1);
         mbar_init(qfull, hasB ? 8 : 4);
-        for (int x = 0; x < 2; ++x) mbar_init(sfull(x), 1), mbar_init(pfull(x), 4), mbar_init(pfull(x) + 16, 4), mbar_init(pvdone(x), 1), mbar_init(ofull(x), 1);
-        mbar_init(mma_done, 1);
+        for (int x = 0; x < 2; ++x) {
+            for (int b = 0; b < 2; ++b) mbar_init(sfull(x, b), 1), mbar_init(pfull(x, b), 4), mbar_init(pvdone(x, b), 1);
+            mbar_init(ofull(x), 1);
+        }
+        mbar_init(mma_done, hasB ? 2 : 1);
         s_abort = 0;
         fence_mbar_init();
     }
@@ -311,127 +319,102 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
 
     if (warp >= kWarpLd) {
         // ------------------------------------------------------------- loads
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         const int w = warp - kWarpLd;
         constexpr int CH = HD / 8, RPI = 32 / CH;       // pieces per row, rows per instruction
         constexpr int NI = kKeys / (kLdWarps * RPI);    // instructions per tile and warp
+        static_assert(NI * RPI == 16, "a warp loads 16 rows of a tile");
         const int ch = lane % CH, rsub = lane / CH, chunks = a.hd / 8;
-        // piece ch of row r of a tile: half ch / 8, row r, piece (ch % 8) ^ (r % 8)
-        auto place = [&](int r) { return (uint32_t)((ch >> 3) * C::HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4)); };
-        // each lane looks up NI * RPI / 32 rows of the warp's share: lane l those of i = l / RPI + 32 / RPI * k
-        constexpr int NL = NI * RPI / 32;
-        static_assert(NL >= 1 && NI * RPI % 32 == 0, "one lookup or more per lane");
-        int64_t off[NL];
-        auto lookup = [&](int x) {
-            const int k0 = tile_key(x);
-#pragma unroll
-            for (int k = 0; k < NL; ++k) {
-                const int i = lane / RPI + k * (32 / RPI);
-                const int j = k0 + (i * kLdWarps + w) * RPI + lane % RPI;
-                off[k] = j < tl.sink_end || (j >= tl.lo && j < tl.hi) ? row_offset(a, s, j, h) : -1;
+        // lanes 0-15 look up the warp's rows of tile xa, lanes 16-31 those of tile xb
+        int64_t off = -1;
+        auto lookup = [&](int xa, int xb) {
+            const int x = lane < 16 ? xa : xb, r = lane & 15;
+            off = -1;
+            if (x < nt) {
+                const int j = tile_key(x0 + x) + ((r / RPI) * kLdWarps + w) * RPI + r % RPI;
+                if (j < tl.sink_end || (j >= tl.lo && j < tl.hi)) off = row_offset(a, s, j, h);
             }
         };
-        lookup(x0);
-        bool ok = true;
-        for (int n = 0; n < 2 * nt && ok; ++n) {
+        lookup(0, 1);
+        for (int n = 0; n <= nt; ++n) {
             const int st = n % C::NST;
-            if (!__all_sync(0xffffffffu, wait_bar(empty(st), ((n / C::NST) & 1) ^ 1, abort, kWtEmpty, p.wait_ns))) {
-                ok = false;
-                break;
-            }
-            const uint16_t* pool = (n & 1) ? a.v : a.k;
-            const uint32_t dst = sbase + C::RING + st * C::TILE;
+            if (!__all_sync(0xffffffffu, wait_bar(empty(st), ((n / C::NST) & 1) ^ 1, abort, kWtEmpty, p.wait_ns))) break;
+            const uint32_t dst = sbase + C::RING + st * C::STAGE + (ch >> 3) * C::HALF;
 #pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                const int r = (i * kLdWarps + w) * RPI + rsub;
-                const int64_t o = __shfl_sync(0xffffffffu, off[i / (32 / RPI)], (i % (32 / RPI)) * RPI + rsub);
-                const bool take = o >= 0 && ch < chunks;
-                cp16(dst + place(r), pool + (take ? o + ch * 8 : 0), take);
+            for (int u = 0; u < 2; ++u) {
+                if (u && n + 1 >= nt) break;  // no tile n + 1
+                const uint16_t* pool = n && !u ? a.v : a.k;
+#pragma unroll
+                for (int i = 0; i < NI; ++i) {
+                    const int r = (i * kLdWarps + w) * RPI + rsub;
+                    const int64_t o = __shfl_sync(0xffffffffu, off, u * 16 + i * RPI + rsub);
+                    const bool take = o >= 0 && ch < chunks;
+                    cp16(dst + u * C::TILE + r * 128 + (((ch & 7) ^ (r & 7)) << 4), pool + (take ? o + ch * 8 : 0), take);
+                }
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            if ((n & 1) && n + 1 < 2 * nt) lookup(x0 + (n + 1) / 2);
-            // the load before this one has landed: hand it to the tensor cores
-            if (n == 0) continue;
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full((n - 1) % C::NST));
+            // the barrier counts this thread's pieces when they have landed
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full(st)) : "memory");
+            lookup(n, n + 2);  // of the next stage: V of tile n, K of tile n + 2
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (ok && lane == 0) mbar_arrive(full((2 * nt - 1) % C::NST));
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp >= kWarpMma) {
         // ---------------------------------------------------------- products
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (warp == kWarpMma) {
-            const uint32_t id_qk = idesc16<DT>(128, kKeys, false), id_pv = idesc16<DT>(128, HD, true);
-            const int nx = hasB ? 2 : 1;
+        const int x = warp - kWarpMma;
+        if (x < (hasB ? 2 : 1)) {
+            const uint32_t id_qk = idesc16<DT>(kM, kKeys, false), id_pv = idesc16<DT>(kM, HD, true);
+            const uint64_t qd = sw128_desc(sbase + x * C::QTILE), kd0 = sw128_desc(sbase + C::RING),
+                           vd0 = sw128_desc_n(sbase + C::RING, C::HALF);
             auto wait = [&](uint32_t bar, int par, int code) {
                 return __all_sync(0xffffffffu, wait_bar(bar, par & 1, abort, code, p.wait_ns));
             };
-            auto qk = [&](int x, int st) {
-                const uint64_t qd = sw128_desc(sbase + x * C::TILE), kd = sw128_desc(sbase + C::RING + st * C::TILE);
+            // S of buffer b from the K tile at `at` (in descriptor units from the ring's start)
+            auto qk = [&](int b, int at) {
 #pragma unroll
-                for (int kk = 0; kk < HD / 16; ++kk) {
-                    const uint64_t step = (uint64_t)((kk >> 2) * (C::HALF >> 4) + 2 * (kk & 3));
-                    tc_mma_f16(tmem + x * kKeys, qd + step, kd + step, id_qk, kk != 0);
-                }
-                tc_commit(sfull(x));
-            };
-            auto pv = [&](int x, int st, int half, bool first) {
-                const uint64_t vd = sw128_desc_n(sbase + C::RING + st * C::TILE, C::HALF);
-                const uint32_t o = tmem + C::O + x * 128;
-#pragma unroll
-                for (int i = 0; i < kKeys / 32; ++i) {
-                    const int kk = half * (kKeys / 32) + i;
-                    tc_mma_f16_ts(o, tmem + x * kKeys + kk * 8, vd + kk * (2048 >> 4), id_pv, !(first && i == 0));
-                }
-                if (precise) {
-#pragma unroll
-                    for (int i = 0; i < kKeys / 32; ++i) {
-                        const int kk = half * (kKeys / 32) + i;
-                        tc_mma_f16_ts(o, tmem + x * kKeys + 64 + kk * 8, vd + kk * (2048 >> 4), id_pv, 1);
-                    }
-                }
+                for (int kk = 0; kk < HD / 16; ++kk)
+                    tc_mma_f16(tmem + x * 128 + b * 64, qd + (uint64_t)((kk >> 2) * (C::QHALF >> 4) + 2 * (kk & 3)),
+                               kd0 + at + (uint64_t)((kk >> 2) * (C::HALF >> 4) + 2 * (kk & 3)), id_qk, kk != 0);
+                tc_commit(sfull(x, b));
             };
             bool ok = wait(qfull, 0, kWtQ) && wait(full(0), 0, kWtFull);
+            fence_proxy_async_smem();
             tc_fence_after();
             if (ok && elect_one()) {
-                for (int x = 0; x < nx; ++x) qk(x, 0);
+                qk(0, 0);
+                if (nt > 1) qk(1, C::TILE >> 4);
                 tc_commit(empty(0));
             }
             __syncwarp();
             for (int j = 0; j < nt && ok; ++j) {
-                const int vn = 2 * j + 1, vs = vn % C::NST, kn = vn + 1, ks = kn % C::NST;
-                ok = wait(full(vs), vn / C::NST, kWtFull);
-                const bool more = j + 1 < nt;
-                for (int x = 0; x < nx && ok; ++x) {
-                    ok = wait(pfull(x), j, kWtP);
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (elect_one()) pv(x, vs, 0, j == 0);
-                    __syncwarp();
-                    ok = wait(pfull(x) + 16, j, kWtP);
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (elect_one()) {
-                        pv(x, vs, 1, false);
-                        tc_commit(more ? pvdone(x) : ofull(x));
-                        if (x == nx - 1) tc_commit(empty(vs));
+                const int b = j & 1, par = (j >> 1) & 1, st = (j + 1) % C::NST;
+                ok = wait(full(st), (j + 1) / C::NST, kWtFull) && wait(pfull(x, b), par, kWtP);
+                if (!ok) break;
+                fence_proxy_async_smem();
+                tc_fence_after();
+                const int at = st * (C::STAGE >> 4);
+                if (elect_one()) {
+                    const uint32_t o = tmem + C::O + x * 128, pp = tmem + x * 128 + b * 64;
+#pragma unroll
+                    for (int kk = 0; kk < kKeys / 16; ++kk)
+                        tc_mma_f16_ts(o, pp + kk * 8, vd0 + at + kk * (2048 >> 4), id_pv, (j | kk) != 0);
+                    if (precise) {
+#pragma unroll
+                        for (int kk = 0; kk < kKeys / 16; ++kk)
+                            tc_mma_f16_ts(o, pp + 32 + kk * 8, vd0 + at + kk * (2048 >> 4), id_pv, 1);
                     }
-                    __syncwarp();
-                    if (!more) continue;
-                    // S of the next tile takes P's columns: the product that reads them must be done
-                    ok = (x > 0 || wait(full(ks), kn / C::NST, kWtFull)) && wait(pvdone(x), j, kWtPv);
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (elect_one()) {
-                        qk(x, ks);
-                        if (x == nx - 1) tc_commit(empty(ks));
-                    }
-                    __syncwarp();
+                    tc_commit(pvdone(x, b));
+                    if (j + 1 == nt) tc_commit(ofull(x));
+                    if (j + 2 >= nt) tc_commit(empty(st));
                 }
+                __syncwarp();
+                if (j + 2 >= nt) continue;
+                // S of the tile after the next takes P's columns: the products that read them must be done
+                ok = wait(pvdone(x, b), par, kWtPv);
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    qk(b, at + (C::TILE >> 4));
+                    tc_commit(empty(st));
+                }
+                __syncwarp();
             }
             // every product has finished before the CTA frees its tensor memory, also when a role gave up
             if (elect_one()) tc_commit(mma_done);
@@ -442,23 +425,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
         }
     } else if (warp < 4 || hasB) {
         // ----------------------------------------------------------- softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
-        const int x = warp >> 2, r = x * kKeys + (warp & 3) * 32 + lane;
+        const int x = warp >> 2, r = x * kM + (warp & 3) * 32 + lane;
         const uint32_t tq = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const uint32_t ts = tq + x * kKeys, to = tq + C::O + x * 128;
+        const uint32_t to = tq + C::O + x * 128;
         const bool valid = r < rows;
         {
             // the warp's 32 rows of Q: piece ch of row r lies in half ch / 8 at (ch % 8) ^ (r % 8)
             constexpr int CH = HD / 8, RPI = 32 / CH;
-            const int ch = lane % CH, r0 = x * kKeys + (warp & 3) * 32 + lane / CH;
+            const int ch = lane % CH, r0 = x * kM + (warp & 3) * 32 + lane / CH;
             const bool in = ch < a.hd / 8;
 #pragma unroll 8
             for (int k = 0; k < CH; ++k) {
-                const int rr = r0 + k * RPI, rt = rr - x * kKeys;
+                const int rr = r0 + k * RPI, rt = rr - x * kM;
                 const bool take = in && rr < rows;
                 int tt = 0;
                 const int hh = take ? row_of(a, p.group_magic, q0, h, R0 + rr, &tt) : 0;
-                cp16(sbase + x * C::TILE + (ch >> 3) * C::HALF + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4),
+                cp16(sbase + x * C::QTILE + (ch >> 3) * C::QHALF + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4),
                      p.q + (take ? tt * p.q_stride + (int64_t)hh * a.hd + ch * 8 : 0), take);
             }
             asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
@@ -478,7 +460,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
         float m0 = -INFINITY, m = -INFINITY, l = 0.0f;  // running maximum of q . k; the one in use, scaled
         bool ok = true;
         for (int j = 0; j < nt; ++j) {
-            if (!__all_sync(0xffffffffu, wait_bar(sfull(x), j & 1, abort, kWtS, p.wait_ns))) {
+            const int b = j & 1;
+            const uint32_t ts = tq + x * 128 + b * 64;
+            if (!__all_sync(0xffffffffu, wait_bar(sfull(x, b), (j >> 1) & 1, abort, kWtS, p.wait_ns))) {
                 ok = false;
                 break;
             }
@@ -508,6 +492,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
                 m = mn;
                 l *= corr;
                 if (j > 0) {
+                    // the product of the tile before this one may still be adding to O
+                    if (!__all_sync(0xffffffffu, wait_bar(pvdone(x, b ^ 1), ((j - 1) >> 1) & 1, abort, kWtPv, p.wait_ns))) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
 #pragma unroll
                     for (int c = 0; c < HD; c += 16) {
                         float o[16];
@@ -522,31 +512,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
             }
             const float ref = m == -INFINITY ? 0.0f : m;
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            uint32_t w[kKeys / 2];
 #pragma unroll
-            for (int c0 = 0; c0 < kKeys; c0 += 64) {
-                uint32_t w[32];
+            for (int c = 0; c < kKeys; c += 2) {
+                fma2(v[c], v[c + 1], p.scale_log2, -ref);
+                v[c] = ex2(v[c]), v[c + 1] = ex2(v[c + 1]);
+                add2(sum[c & 2], sum[(c & 2) + 1], v[c], v[c + 1]);
+                w[c / 2] = X::pack(v[c], v[c + 1]);
+            }
+            tmem_st32(ts, w);
+            if (precise) {
 #pragma unroll
-                for (int c = 0; c < 64; c += 2) {
-                    float &a0 = v[c0 + c], &a1 = v[c0 + c + 1];
-                    fma2(a0, a1, p.scale_log2, -ref);
-                    a0 = ex2(a0), a1 = ex2(a1);
-                    add2(sum[c & 2], sum[(c & 2) + 1], a0, a1);
-                    w[c / 2] = X::pack(a0, a1);
-                }
-                tmem_st32(ts + c0 / 2, w);
-                if (precise) {
-#pragma unroll
-                    for (int c = 0; c < 64; c += 2)
-                        w[c / 2] = X::pack(v[c0 + c] - X::lo(w[c / 2]), v[c0 + c + 1] - X::hi(w[c / 2]));
-                    tmem_st32(ts + 64 + c0 / 2, w);
-                }
-                // half of the positions: their products may start
-                tc_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(pfull(x) + (c0 ? 16 : 0));
+                for (int c = 0; c < kKeys; c += 2) w[c / 2] = X::pack(v[c] - X::lo(w[c / 2]), v[c + 1] - X::hi(w[c / 2]));
+                tmem_st32(ts + 32, w);
             }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(pfull(x, b));
         }
         // ------------------------------------------------------- the rows out
         ok = ok && __all_sync(0xffffffffu, wait_bar(ofull(x), 0, abort, kWtO, p.wait_ns));
@@ -555,28 +539,31 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
             const int64_t row = (int64_t)t * nq + head;
             bool bad = false;
             if (split && valid) p.part_ml[(int64_t)z * p.T * nq + row] = make_float2(m, l);
-            float o[HD];
+            const float inv = i < 0 ? 0.0f : 1.0f / l;
 #pragma unroll
-            for (int c = 0; c < HD; c += 32) tmem_ld32(to + c, o + c);
-            tc_wait_ld();
-            if (split) {
-                float4* dst = reinterpret_cast<float4*>(p.part_acc + ((int64_t)z * p.T * nq + row) * HD);
-                if (valid)
+            for (int c = 0; c < HD; c += 64) {
+                float o[64];
+                tmem_ld32(to + c, o);
+                tmem_ld32(to + c + 32, o + 32);
+                tc_wait_ld();
+                if (split) {
+                    float4* dst = reinterpret_cast<float4*>(p.part_acc + ((int64_t)z * p.T * nq + row) * HD + c);
+                    if (valid)
 #pragma unroll
-                    for (int e = 0; e < HD / 4; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-            } else {
-                const float inv = i < 0 ? 0.0f : 1.0f / l;
+                        for (int e = 0; e < 16; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                } else {
 #pragma unroll
-                for (int e = 0; e < HD; e += 8) {
-                    float y[8];
+                    for (int e = 0; e < 64; e += 8) {
+                        float y[8];
 #pragma unroll
-                    for (int b = 0; b < 8; ++b) {
-                        y[b] = i < 0 ? 0.0f : o[e + b] * inv;
-                        bad |= !(fabsf(y[b]) <= 3.4e38f);
+                        for (int b = 0; b < 8; ++b) {
+                            y[b] = i < 0 ? 0.0f : o[e + b] * inv;
+                            bad |= !(fabsf(y[b]) <= 3.4e38f);
+                        }
+                        if (valid && c + e < a.hd)
+                            *reinterpret_cast<uint4*>(p.out + row * a.hd + c + e) =
+                                make_uint4(X::pack(y[0], y[1]), X::pack(y[2], y[3]), X::pack(y[4], y[5]), X::pack(y[6], y[7]));
                     }
-                    if (valid && e < a.hd)
-                        *reinterpret_cast<uint4*>(p.out + row * a.hd + e) =
-                            make_uint4(X::pack(y[0], y[1]), X::pack(y[2], y[3]), X::pack(y[4], y[5]), X::pack(y[6], y[7]));
                 }
             }
             uint32_t again = __ballot_sync(0xffffffffu, bad && valid);
@@ -587,8 +574,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
                                   __shfl_sync(0xffffffffu, i, who));
             }
         }
-    } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     }
     tc_fence_before();
     __syncthreads();
