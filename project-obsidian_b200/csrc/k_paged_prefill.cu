@@ -22,6 +22,9 @@
 //              thread's row.  O is rescaled only when the maximum has grown by more
 //              than 2^8 (p stays below 2^8, far inside both types), by the same
 //              threads, between a tile's S and its P, when no product touches O
+//              The two tiles' warps of one scheduler take turns at the exponentials: in
+//              step they would share the exponential unit and then leave it idle, and
+//              both tiles' products would queue up behind one another
 //   8, 9       issue the products of tile A, of tile B: PV of a tile of positions, then
 //              QK of the tile after the next into the columns that this P leaves
 //   12-15      loads: rows of K and V by page, 16 bytes per cp.async, into the
@@ -65,12 +68,12 @@ struct Pf {
     static constexpr int NST = HD == 128 ? 4 : 8;
     static constexpr int RING = 2 * QTILE;
     static constexpr int BAR = RING + NST * STAGE;
-    static constexpr int NBAR = 2 * NST + 1 + 2 * 7 + 1;
+    static constexpr int NBAR = 2 * NST + 1 + 2 * 7 + 1 + 8;
     static constexpr int SMEM = BAR + NBAR * 8 + 1024;
     static constexpr int O = 256;                     // TMEM: S of tile x, buffer b at 128 x + 64 b; O at 256 + 128 x
 };
 
-enum Wait : int { kWtEmpty = 31, kWtFull, kWtQ, kWtS, kWtP, kWtPv, kWtO };
+enum Wait : int { kWtEmpty = 31, kWtFull, kWtQ, kWtS, kWtP, kWtPv, kWtO, kWtTurn };
 
 // mbar_wait without the suspend hint (waits here are shorter than waking up takes)
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile int* abort, int code,
@@ -220,6 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
     auto pvdone = [&](int x, int b) { return qfull + 72 + 8 * (2 * x + b); };
     auto ofull = [&](int x) { return qfull + 104 + 8 * x; };
     const uint32_t mma_done = qfull + 120;
+    auto turn = [&](int x, int w) { return qfull + 128 + 8 * (4 * x + w); };
     const PagedArgs& a = p.c;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     volatile int* abort = &s_abort;
@@ -305,6 +309,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
             mbar_init(ofull(x), 1);
         }
         mbar_init(mma_done, hasB ? 2 : 1);
+        for (int i = 0; i < 8; ++i) mbar_init(turn(i >> 2, i & 3), 1);
         s_abort = 0;
         fence_mbar_init();
     }
@@ -510,21 +515,33 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
                     }
                 }
             }
+            // the two tiles' warps of one scheduler take turns at the exponentials
+            if (hasB && !__all_sync(0xffffffffu, wait_bar(turn(x, warp & 3), (j & 1) ^ (x == 0), abort, kWtTurn, p.wait_ns))) {
+                ok = false;
+                break;
+            }
             const float ref = m == -INFINITY ? 0.0f : m;
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            uint32_t w[kKeys / 2];
 #pragma unroll
-            for (int c = 0; c < kKeys; c += 2) {
-                fma2(v[c], v[c + 1], p.scale_log2, -ref);
-                v[c] = ex2(v[c]), v[c + 1] = ex2(v[c + 1]);
-                add2(sum[c & 2], sum[(c & 2) + 1], v[c], v[c + 1]);
-                w[c / 2] = X::pack(v[c], v[c + 1]);
-            }
-            tmem_st32(ts, w);
-            if (precise) {
+            for (int c0 = 0; c0 < kKeys; c0 += 32) {
+                uint32_t w[16];
 #pragma unroll
-                for (int c = 0; c < kKeys; c += 2) w[c / 2] = X::pack(v[c] - X::lo(w[c / 2]), v[c + 1] - X::hi(w[c / 2]));
-                tmem_st32(ts + 32, w);
+                for (int c = 0; c < 32; c += 2) {
+                    float &a0 = v[c0 + c], &a1 = v[c0 + c + 1];
+                    fma2(a0, a1, p.scale_log2, -ref);
+                    a0 = ex2(a0), a1 = ex2(a1);
+                    add2(sum[c & 2], sum[(c & 2) + 1], a0, a1);
+                    w[c / 2] = X::pack(a0, a1);
+                }
+                tmem_st16(ts + c0 / 2, w);
+                // (handing over takes as long as the second half)
+                if (c0 == 0 && hasB && lane == 0) mbar_arrive(turn(x ^ 1, warp & 3));
+                if (precise) {
+#pragma unroll
+                    for (int c = 0; c < 32; c += 2)
+                        w[c / 2] = X::pack(v[c0 + c] - X::lo(w[c / 2]), v[c0 + c + 1] - X::hi(w[c / 2]));
+                    tmem_st16(ts + 32 + c0 / 2, w);
+                }
             }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             tc_wait_st();
