@@ -228,6 +228,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     volatile int* abort = &s_abort;
 
+    if (warp == kWarpMma) {  // (under the loads of the search)
+        tmem_alloc(smem_u32(&s_tmem), 512);
+        tmem_relinquish();
+    }
     // ---- which block of rows: blocks of all the sequences in one line, the last
     // (the longest of their sequence) first; the KV heads of a block side by side
     const int h = blockIdx.x % a.nkv, bi = blockIdx.x / a.nkv, z = blockIdx.y;
@@ -276,7 +280,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
         __syncthreads();
     }
     const int s = s_blk[0];
-    if (s < 0) return;
+    if (s < 0) {
+        if (warp == kWarpMma) tmem_dealloc(s_tmem, 512);
+        return;
+    }
     const int q0 = s_blk[2], nrow = (s_blk[3] - q0) * a.group;
     const int R0 = s_blk[1] * kRows, rows = min(kRows, nrow - R0);
     const bool hasB = rows > kM;
@@ -295,27 +302,78 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
                 for (int d = 0; d < a.hd; d += 8)
                     *reinterpret_cast<uint4*>(p.out + ((int64_t)t * nq + head) * a.hd + d) = make_uint4(0, 0, 0, 0);
         }
+        if (warp == kWarpMma) tmem_dealloc(s_tmem, 512);
         return;
     }
     const int x0 = (int)((int64_t)tl.nt * z / ns), x1 = (int)((int64_t)tl.nt * (z + 1) / ns), nt = x1 - x0;
     auto tile_key = [&](int x) { return (x < tl.ts ? x : x - tl.ts + tl.wt) * kKeys; };
     const bool precise = i_lo < 0 || seen(i_lo, p.window, p.n_sink) < kFewKeys;
 
-    if (tid == 0) {
-        for (int i = 0; i < C::NST; ++i) mbar_init(full(i), 32 * kLdWarps), mbar_init(empty(i), hasB ? 2 : 1);
-        mbar_init(qfull, hasB ? 8 : 4);
-        for (int x = 0; x < 2; ++x) {
-            for (int b = 0; b < 2; ++b) mbar_init(sfull(x, b), 1), mbar_init(pfull(x, b), 4), mbar_init(pvdone(x, b), 1);
-            mbar_init(ofull(x), 1);
+    if (warp == kWarpMma + 1) {
+        // the barriers in the order of their places; two of a kind for the two row tiles
+        const int nx = hasB ? 2 : 1;
+        for (int i = lane; i < C::NBAR; i += 32) {
+            const int k = i - 2 * C::NST;
+            const int count = i < C::NST ? 32 * kLdWarps                   // full
+                              : k < 0 ? nx                                 // empty
+                              : k == 0 ? 4 * nx                            // Q
+                              : k >= 5 && k < 9 ? 4                        // P
+                              : k == 15 ? nx                               // the last products
+                                        : 1;                               // S, PV done, O, turns
+            mbar_init(bars + 8 * i, count);
         }
-        mbar_init(mma_done, hasB ? 2 : 1);
-        for (int i = 0; i < 8; ++i) mbar_init(turn(i >> 2, i & 3), 1);
-        s_abort = 0;
+        if (lane == 0) s_abort = 0;
         fence_mbar_init();
     }
-    if (warp == kWarpMma) {
-        tmem_alloc(smem_u32(&s_tmem), 512);
-        tmem_relinquish();
+    // ---- the first loads, then everybody's barriers and tensor memory
+    constexpr int CH = HD / 8, RPI = 32 / CH;       // 16-byte pieces per row, rows per instruction
+    constexpr int NI = kKeys / (kLdWarps * RPI);    // instructions per tile and loading warp
+    static_assert(NI * RPI == 16, "a loading warp takes 16 rows of a tile");
+    const int ch = lane % CH, rsub = lane / CH, chunks = a.hd / 8;
+    int64_t off = -1;
+    // lanes 0-15 look up the warp's rows of tile xa, lanes 16-31 those of tile xb
+    auto lookup = [&](int xa, int xb) {
+        const int x = lane < 16 ? xa : xb, r = lane & 15;
+        off = -1;
+        if (x < nt) {
+            const int j = tile_key(x0 + x) + ((r / RPI) * kLdWarps + warp - kWarpLd) * RPI + r % RPI;
+            if (j < tl.sink_end || (j >= tl.lo && j < tl.hi)) off = row_offset(a, s, j, h);
+        }
+    };
+    auto load_stage = [&](int n) {
+        const uint32_t dst = sbase + C::RING + (n % C::NST) * C::STAGE + (ch >> 3) * C::HALF;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            if (u && n + 1 >= nt) break;  // no tile n + 1
+            const uint16_t* pool = n && !u ? a.v : a.k;
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int r = (i * kLdWarps + warp - kWarpLd) * RPI + rsub;
+                const int64_t o = __shfl_sync(0xffffffffu, off, u * 16 + i * RPI + rsub);
+                const bool take = o >= 0 && ch < chunks;
+                cp16(dst + u * C::TILE + r * 128 + (((ch & 7) ^ (r & 7)) << 4), pool + (take ? o + ch * 8 : 0), take);
+            }
+        }
+    };
+    if (warp >= kWarpLd) {
+        lookup(0, 1);
+        load_stage(0);
+    } else if (warp < (hasB ? 8 : 4)) {
+        // the warp's 32 rows of Q: piece ch of row r lies in half ch / 8 at (ch % 8) ^ (r % 8);
+        // lane l knows where row l of them is
+        const int r = warp * 32 + lane;
+        int t;
+        const int head = row_of(a, p.group_magic, q0, h, R0 + min(r, rows - 1), &t);
+        const int64_t at = r < rows ? t * p.q_stride + (int64_t)head * a.hd : -1;
+#pragma unroll
+        for (int k = 0; k < CH; ++k) {
+            const int rr = k * RPI + rsub, rt = (warp & 3) * 32 + rr;
+            const int64_t o = __shfl_sync(0xffffffffu, at, rr);
+            const bool take = o >= 0 && ch < chunks;
+            cp16(sbase + (warp >> 2) * C::QTILE + (ch >> 3) * C::QHALF + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4),
+                 p.q + (take ? o + ch * 8 : 0), take);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
@@ -324,37 +382,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
 
     if (warp >= kWarpLd) {
         // ------------------------------------------------------------- loads
-        const int w = warp - kWarpLd;
-        constexpr int CH = HD / 8, RPI = 32 / CH;       // pieces per row, rows per instruction
-        constexpr int NI = kKeys / (kLdWarps * RPI);    // instructions per tile and warp
-        static_assert(NI * RPI == 16, "a warp loads 16 rows of a tile");
-        const int ch = lane % CH, rsub = lane / CH, chunks = a.hd / 8;
-        // lanes 0-15 look up the warp's rows of tile xa, lanes 16-31 those of tile xb
-        int64_t off = -1;
-        auto lookup = [&](int xa, int xb) {
-            const int x = lane < 16 ? xa : xb, r = lane & 15;
-            off = -1;
-            if (x < nt) {
-                const int j = tile_key(x0 + x) + ((r / RPI) * kLdWarps + w) * RPI + r % RPI;
-                if (j < tl.sink_end || (j >= tl.lo && j < tl.hi)) off = row_offset(a, s, j, h);
-            }
-        };
-        lookup(0, 1);
         for (int n = 0; n <= nt; ++n) {
             const int st = n % C::NST;
-            if (!__all_sync(0xffffffffu, wait_bar(empty(st), ((n / C::NST) & 1) ^ 1, abort, kWtEmpty, p.wait_ns))) break;
-            const uint32_t dst = sbase + C::RING + st * C::STAGE + (ch >> 3) * C::HALF;
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                if (u && n + 1 >= nt) break;  // no tile n + 1
-                const uint16_t* pool = n && !u ? a.v : a.k;
-#pragma unroll
-                for (int i = 0; i < NI; ++i) {
-                    const int r = (i * kLdWarps + w) * RPI + rsub;
-                    const int64_t o = __shfl_sync(0xffffffffu, off, u * 16 + i * RPI + rsub);
-                    const bool take = o >= 0 && ch < chunks;
-                    cp16(dst + u * C::TILE + r * 128 + (((ch & 7) ^ (r & 7)) << 4), pool + (take ? o + ch * 8 : 0), take);
-                }
+            if (n) {
+                if (!__all_sync(0xffffffffu, wait_bar(empty(st), ((n / C::NST) & 1) ^ 1, abort, kWtEmpty, p.wait_ns))) break;
+                load_stage(n);
             }
             // the barrier counts this thread's pieces when they have landed
             asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full(st)) : "memory");
@@ -434,25 +466,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
         const uint32_t tq = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t to = tq + C::O + x * 128;
         const bool valid = r < rows;
-        {
-            // the warp's 32 rows of Q: piece ch of row r lies in half ch / 8 at (ch % 8) ^ (r % 8)
-            constexpr int CH = HD / 8, RPI = 32 / CH;
-            const int ch = lane % CH, r0 = x * kM + (warp & 3) * 32 + lane / CH;
-            const bool in = ch < a.hd / 8;
-#pragma unroll 8
-            for (int k = 0; k < CH; ++k) {
-                const int rr = r0 + k * RPI, rt = rr - x * kM;
-                const bool take = in && rr < rows;
-                int tt = 0;
-                const int hh = take ? row_of(a, p.group_magic, q0, h, R0 + rr, &tt) : 0;
-                cp16(sbase + x * C::QTILE + (ch >> 3) * C::QHALF + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4),
-                     p.q + (take ? tt * p.q_stride + (int64_t)hh * a.hd + ch * 8 : 0), take);
-            }
-            asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(qfull);
-        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(qfull);
         int t;
         const int head = row_of(a, p.group_magic, q0, h, R0 + min(r, rows - 1), &t);
         const int i = base + (t - q0), lo = window_lo(i, p.window);
@@ -555,6 +572,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
             tc_fence_after();
             const int64_t row = (int64_t)t * nq + head;
             bool bad = false;
+            uint8_t* stg = smem + x * C::QTILE + (warp & 3) * 4096;
             if (split && valid) p.part_ml[(int64_t)z * p.T * nq + row] = make_float2(m, l);
             const float inv = i < 0 ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -569,17 +587,28 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
 #pragma unroll
                         for (int e = 0; e < 16; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                 } else {
+// through shared memory (Q's rows of this warp, which no product needs any more), so
+                    // that a store writes whole lines: piece e of row lane lies at e ^ (lane % 8)
+                    __syncwarp();
 #pragma unroll
-                    for (int e = 0; e < 64; e += 8) {
+                    for (int e = 0; e < 8; ++e) {
                         float y[8];
 #pragma unroll
-                        for (int b = 0; b < 8; ++b) {
-                            y[b] = i < 0 ? 0.0f : o[e + b] * inv;
-                            bad |= !(fabsf(y[b]) <= 3.4e38f);
+                        for (int d = 0; d < 8; ++d) {
+                            y[d] = i < 0 ? 0.0f : o[8 * e + d] * inv;
+                            bad |= !(fabsf(y[d]) <= 3.4e38f);
                         }
-                        if (valid && c + e < a.hd)
-                            *reinterpret_cast<uint4*>(p.out + row * a.hd + c + e) =
-                                make_uint4(X::pack(y[0], y[1]), X::pack(y[2], y[3]), X::pack(y[4], y[5]), X::pack(y[6], y[7]));
+                        *reinterpret_cast<uint4*>(stg + lane * 128 + ((e ^ (lane & 7)) << 4)) =
+                            make_uint4(X::pack(y[0], y[1]), X::pack(y[2], y[3]), X::pack(y[4], y[5]), X::pack(y[6], y[7]));
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int rr = e * 4 + (lane >> 3), pc = lane & 7;
+                        const int64_t out_row = __shfl_sync(0xffffffffu, row, rr);
+                        if (x * kM + (warp & 3) * 32 + rr < rows && c + pc * 8 < a.hd)
+                            *reinterpret_cast<uint4*>(p.out + out_row * a.hd + c + pc * 8) =
+                                *reinterpret_cast<const uint4*>(stg + rr * 128 + ((pc ^ (rr & 7)) << 4));
                     }
                 }
             }
