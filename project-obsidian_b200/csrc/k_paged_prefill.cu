@@ -108,6 +108,15 @@ __device__ __forceinline__ void fma2(float& a0, float& a1, float s, float c) {
         : "+f"(a0), "+f"(a1)
         : "f"(s), "f"(c));
 }
+// two at once: a * b + c
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
 __device__ __forceinline__ void add2(float& s0, float& s1, float a0, float a1) {
     asm("{\n\t.reg .b64 s, a;\n\tmov.b64 s, {%0, %1};\n\tmov.b64 a, {%2, %3};\n\tadd.rn.f32x2 s, s, a;\n\t"
         "mov.b64 {%0, %1}, s;\n\t}"
@@ -235,14 +244,36 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
     // ---- which block of rows: blocks of all the sequences in one line, the last
     // (the longest of their sequence) first; the KV heads of a block side by side
     const int h = blockIdx.x % a.nkv, bi = blockIdx.x / a.nkv, z = blockIdx.y;
-    {
+    int s = -1, blk = 0, q0 = 0, q1 = 0, len = 0;
+    if (a.n_seqs <= 32) {
+        // every warp for itself, a sequence per lane
+        const bool in = lane < a.n_seqs;
+        const int lq0 = in ? p.q_start[lane] : 0, lq1 = in ? p.q_start[lane + 1] : 0, ll = in ? seq_len(a, lane) : 0;
+        const bool ok = lq0 >= 0 && lq1 >= lq0 && lq1 <= p.T && (lane > 0 || lq0 == 0) &&
+                        (lane != a.n_seqs - 1 || lq1 == p.T);
+        if (!ok && tid == lane) atomicExch(a.err, kDevBadPos);
+        const int mine = ok ? ((lq1 - lq0) * a.group + kRows - 1) / kRows : 0;
+        int incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        const int want = __shfl_sync(0xffffffffu, incl, 31) - 1 - bi;
+        const uint32_t who = __ballot_sync(0xffffffffu, want >= incl - mine && want < incl);
+        if (who) {
+            s = __ffs(who) - 1;
+            blk = want - __shfl_sync(0xffffffffu, incl - mine, s);
+            q0 = __shfl_sync(0xffffffffu, lq0, s), q1 = __shfl_sync(0xffffffffu, lq1, s);
+            len = __shfl_sync(0xffffffffu, ll, s);
+        }
+    } else {
         const int per = (a.n_seqs + kThreads - 1) / kThreads;
         const int sb = min(a.n_seqs, tid * per), se = min(a.n_seqs, sb + per);
-        int mine = 0, len0 = 0, q0 = 0, q1 = 0;  // of the thread's first sequence, at hand when it is the block's
+        int mine = 0;
         bool bad = tid == 0 && (p.q_start[0] != 0 || p.q_start[a.n_seqs] != p.T);
-        for (int s = sb; s < se; ++s) {
-            const int b0 = p.q_start[s], b1 = p.q_start[s + 1];
-            if (s == sb) len0 = seq_len(a, s), q0 = b0, q1 = b1;
+        for (int i = sb; i < se; ++i) {
+            const int b0 = p.q_start[i], b1 = p.q_start[i + 1];
             if (b0 < 0 || b1 < b0 || b1 > p.T) bad = true;
             else mine += ((b1 - b0) * a.group + kRows - 1) / kRows;
         }
@@ -265,30 +296,31 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
         const int want = total - 1 - bi;
         if (want >= before && want < before + mine) {
             int b = before;
-            for (int s = sb; s < se; ++s) {
-                if (s > sb) q0 = p.q_start[s], q1 = p.q_start[s + 1];
-                if (q0 < 0 || q1 < q0 || q1 > p.T) continue;
-                const int c = ((q1 - q0) * a.group + kRows - 1) / kRows;
+            for (int i = sb; i < se; ++i) {
+                const int b0 = p.q_start[i], b1 = p.q_start[i + 1];
+                if (b0 < 0 || b1 < b0 || b1 > p.T) continue;
+                const int c = ((b1 - b0) * a.group + kRows - 1) / kRows;
                 if (want < b + c) {
-                    s_blk[0] = s, s_blk[1] = want - b, s_blk[2] = q0, s_blk[3] = q1;
-                    s_blk[4] = s == sb ? len0 : seq_len(a, s);
+                    s_blk[0] = i, s_blk[1] = want - b, s_blk[2] = b0, s_blk[3] = b1, s_blk[4] = seq_len(a, i);
                     break;
                 }
                 b += c;
             }
         }
         __syncthreads();
+        s = s_blk[0], blk = s_blk[1], q0 = s_blk[2], q1 = s_blk[3], len = s_blk[4];
     }
-    const int s = s_blk[0];
     if (s < 0) {
+        __syncthreads();
         if (warp == kWarpMma) tmem_dealloc(s_tmem, 512);
         return;
     }
-    const int q0 = s_blk[2], nrow = (s_blk[3] - q0) * a.group;
-    const int R0 = s_blk[1] * kRows, rows = min(kRows, nrow - R0);
+    const int R0 = blk * kRows, rows = min(kRows, (q1 - q0) * a.group - R0);
+    const int base = len - (q1 - q0);  // position of the sequence's first new token
+    int t_lo, t_hi;
+    row_of(a, p.group_magic, base, h, R0, &t_lo), row_of(a, p.group_magic, base, h, R0 + rows - 1, &t_hi);
+    const int i_lo = t_lo, i_hi = t_hi;
     const bool hasB = rows > kM;
-    const int base = s_blk[4] - (s_blk[3] - q0);  // position of the sequence's first new token
-    const int i_lo = base + R0 / a.group, i_hi = base + (R0 + rows - 1) / a.group;
     const Tiles tl = tiles_of(i_lo, i_hi, p.window, p.n_sink);
     const bool split = p.splits > 1;
     const int ns = min(p.splits, tl.nt);
@@ -302,10 +334,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
                 for (int d = 0; d < a.hd; d += 8)
                     *reinterpret_cast<uint4*>(p.out + ((int64_t)t * nq + head) * a.hd + d) = make_uint4(0, 0, 0, 0);
         }
+        __syncthreads();
         if (warp == kWarpMma) tmem_dealloc(s_tmem, 512);
         return;
     }
-    const int x0 = (int)((int64_t)tl.nt * z / ns), x1 = (int)((int64_t)tl.nt * (z + 1) / ns), nt = x1 - x0;
+    // (nt <= 2^14, splits <= the number of SMs)
+    const int x0 = split ? tl.nt * z / ns : 0, nt = (split ? tl.nt * (z + 1) / ns : tl.nt) - x0;
     auto tile_key = [&](int x) { return (x < tl.ts ? x : x - tl.ts + tl.wt) * kKeys; };
     const bool precise = i_lo < 0 || seen(i_lo, p.window, p.n_sink) < kFewKeys;
 
@@ -571,16 +605,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
         if (ok) {
             tc_fence_after();
             const int64_t row = (int64_t)t * nq + head;
-            bool bad = false;
+            float2 fin = make_float2(0.0f, 0.0f);
             uint8_t* stg = smem + x * C::QTILE + (warp & 3) * 4096;
             if (split && valid) p.part_ml[(int64_t)z * p.T * nq + row] = make_float2(m, l);
-            const float inv = i < 0 ? 0.0f : 1.0f / l;
+            const float inv = i < 0 ? 1.0f : 1.0f / l;
 #pragma unroll
             for (int c = 0; c < HD; c += 64) {
                 float o[64];
                 tmem_ld32(to + c, o);
                 tmem_ld32(to + c + 32, o + 32);
                 tc_wait_ld();
+                if (i < 0) {  // nothing to see
+#pragma unroll
+                    for (int e = 0; e < 64; ++e) o[e] = 0.0f;
+                }
                 if (split) {
                     float4* dst = reinterpret_cast<float4*>(p.part_acc + ((int64_t)z * p.T * nq + row) * HD + c);
                     if (valid)
@@ -592,11 +630,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
                     __syncwarp();
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        float y[8];
+                        float* y = o + 8 * e;
 #pragma unroll
-                        for (int d = 0; d < 8; ++d) {
-                            y[d] = i < 0 ? 0.0f : o[8 * e + d] * inv;
-                            bad |= !(fabsf(y[d]) <= 3.4e38f);
+                        for (int d = 0; d < 8; d += 2) {
+                            fma2(y[d], y[d + 1], inv, 0.0f);
+                            fin = fma2(make_float2(y[d], y[d + 1]), make_float2(0.0f, 0.0f), fin);  // NaN once one is not finite
                         }
                         *reinterpret_cast<uint4*>(stg + lane * 128 + ((e ^ (lane & 7)) << 4)) =
                             make_uint4(X::pack(y[0], y[1]), X::pack(y[2], y[3]), X::pack(y[4], y[5]), X::pack(y[6], y[7]));
@@ -612,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
                     }
                 }
             }
-            uint32_t again = __ballot_sync(0xffffffffu, bad && valid);
+            uint32_t again = __ballot_sync(0xffffffffu, valid && i >= 0 && !(fin.x + fin.y == 0.0f) && !split);
             while (again) {  // (never with split: k_paged_join does it)
                 const int who = __ffs(again) - 1;
                 again &= again - 1;
