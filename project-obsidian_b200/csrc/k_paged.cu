@@ -37,21 +37,24 @@ __global__ void __launch_bounds__(256) k_paged_append(PagedArgs a, const uint16_
 
 // ------------------------------------------------------------------ eviction
 // Which positions of (sequence s, KV head h) stay: all n if n <= budget, else the
-// first n_sink, the last n_recent and, of the rest, the budget - n_sink - n_recent
-// with the largest weights (equal weights: the lowest position; NaN lowest of all).
-// A cluster of kEvC CTAs per (s, h):
+// first n_sink, the last n_recent and, of the rest, the `need` = budget - n_sink -
+// n_recent with the largest weights (equal weights: the lowest position; NaN lowest
+// of all), in two launches.
 //   select   radix selection over the weights as ordered 32-bit keys, 11 + 11 + 10
-//            bits from the top: a histogram per CTA in shared memory, summed over
-//            the cluster through distributed shared memory, gives the digit of the
-//            threshold key; then each CTA's part of the positions is counted and
-//            walked in order, which gives every kept position its place.
-//   move     the kept rows to places 0, 1, ... of dst in steps of rows that the
-//            cluster holds in registers: places [c0, c1) come from positions >= c0,
-//            so with a cluster barrier between a step's reads and its writes the
-//            move may be in place (a later step reads positions >= c1 only).
-constexpr int kEvC = 8, kEvThreads = 512, kEvBins = 2048;
+//            bits from the top: a histogram in shared memory gives the digit of the
+//            threshold key.  One CTA holds up to kEvChunk positions in registers; for
+//            longer caches a cluster of kEvC shares them and adds its histograms up
+//            through distributed shared memory.  Ballots then give every kept position
+//            its place, in order.  (Comparing the keys with three candidates a round,
+//            two bits at a time, needs no histogram, but its sixteen rounds took 20 us
+//            where this takes KEEPUS.)
+//   move     the kept rows to places 0, 1, ... of dst.
+constexpr int kEvC = 8, kEvThreads = 512, kEvWarps = kEvThreads / 32;
+constexpr int kEvBins = 2048;
+constexpr int kEvRows = 16, kEvChunk = kEvRows * kEvThreads;  // positions a CTA holds at a time
+static_assert(2 * kEvRows * kEvWarps == kEvThreads, "one thread per entry of s_at");
 
-// larger weight <=> larger key; -0 and +0 equal; NaN the smallest
+// larger weight <=> larger key; -0 and +0 equal; NaN the smallest (0)
 __device__ __forceinline__ uint32_t weight_key(float w) {
     if (w != w) return 0u;
     const uint32_t b = __float_as_uint(w + 0.0f);
@@ -69,9 +72,8 @@ struct EvictArgs {
     int in_place;
 };
 
-// inclusive prefix sum of one value per thread over the CTA; returns the sum over
-// the threads before this one, total in *sum
-__device__ __forceinline__ int block_excl(int v, int* s_warp, int* sum) {
+// exclusive prefix sum over the CTA of one value per thread (two barriers)
+__device__ __forceinline__ int block_excl(int v, int* s_warp) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int x = v;
 #pragma unroll
@@ -82,163 +84,233 @@ __device__ __forceinline__ int block_excl(int v, int* s_warp, int* sum) {
     __syncthreads();
     if (lane == 31) s_warp[warp] = x;
     __syncthreads();
-    if (warp == 0) {
-        int t = lane < kEvThreads / 32 ? s_warp[lane] : 0;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, t, o);
-            if (lane >= o) t += y;
-        }
-        s_warp[lane] = t;
-    }
-    __syncthreads();
-    *sum = s_warp[kEvThreads / 32 - 1];
-    return x - v + (warp ? s_warp[warp - 1] : 0);
+    return x - v + __reduce_add_sync(0xffffffffu, lane < warp ? s_warp[lane] : 0);
 }
 
-__global__ void __cluster_dims__(kEvC, 1, 1) __launch_bounds__(kEvThreads) k_paged_evict(EvictArgs e) {
+__global__ void __launch_bounds__(kEvThreads) k_paged_select(EvictArgs e) {
     pdl_begin();
     cg::cluster_group cl = cg::this_cluster();
-    __shared__ uint32_t s_hist[2][kEvBins];
-    __shared__ int s_warp[32];
-    __shared__ int s_cnt[2];
-    __shared__ uint32_t s_digit, s_above;
+    __shared__ uint32_t s_key[kEvChunk];
+    __shared__ uint32_t s_hist[kEvBins];
+    __shared__ int s_at[2][kEvRows * kEvWarps];  // kept above the threshold / equal to it, by row of 32
+    __shared__ int s_warp[kEvWarps], s_tot[2];
     const PagedArgs& a = e.src;
-    const int rank = (int)cl.block_rank(), h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x;
+    const int rank = (int)cl.block_rank(), size = (int)cl.num_blocks(), h = blockIdx.y, s = blockIdx.z;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int n = seq_len(a, s), m = n < e.budget ? n : e.budget;
     const int64_t row = (int64_t)s * a.nkv + h;
     const float* w = e.w + row * e.w_stride;
     int32_t* kept = e.kept + row * e.budget;
     if (rank == 0 && h == 0 && tid == 0) e.new_len[s] = m;
 
-    if (n <= e.budget) {
-        for (int j = rank * kEvThreads + tid; j < e.budget; j += kEvC * kEvThreads) kept[j] = j < n ? j : -1;
-    } else {
-        const int lo = e.n_sink, hi = n - e.n_recent, need = e.budget - e.n_sink - e.n_recent;
-        const int per = (hi - lo + kEvC - 1) / kEvC;
-        const int b0 = min(hi, lo + rank * per), b1 = min(hi, b0 + per);
-        // the threshold key, digit by digit from the top; `left`: how many of the keys
+    const int all = n <= e.budget;
+    const int lo = all ? n : e.n_sink, hi = all ? n : n - e.n_recent;  // the positions that are chosen from
+    for (int j = rank * kEvThreads + tid; j < e.budget; j += size * kEvThreads) {
+        if (all) kept[j] = j < n ? j : -1;
+        else if (j < lo) kept[j] = j;
+        else if (j >= e.budget - e.n_recent) kept[j] = n - e.budget + j;
+    }
+    const int need = e.budget - e.n_sink - e.n_recent;
+    const int parts = hi - lo <= kEvChunk ? 1 : size;  // CTAs that share them
+    if (!all && need > 0 && rank < parts) {
+        const int per = (hi - lo + parts - 1) / parts;
+        const int b0 = min(hi, lo + rank * per), len = min(hi, b0 + per) - b0;
+        const bool held = len <= kEvChunk;
+        if (held)
+            for (int j = tid; j < len; j += kEvThreads) s_key[j] = weight_key(w[b0 + j]);  // (each thread reads its own)
+        auto key_at = [&](int j) { return j >= len ? 0u : held ? s_key[j] : weight_key(w[b0 + j]); };
+        // (the loops are kept rolled: most of this code runs once, and unrolled it was
+        // waiting for its instructions)
+        // the threshold key t, digit by digit from the top; `left`: how many of the keys
         // that share the digits found so far are kept
-        uint32_t prefix = 0;
+        uint32_t t = 0;
         int left = need;
-        const int shift[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
-#pragma unroll
-        for (int pass = 0; pass < 3; ++pass) {
-            uint32_t* hist = s_hist[pass & 1];
-            const int bins = 1 << bits[pass], sh = shift[pass];
-            for (int i = tid; i < bins; i += kEvThreads) hist[i] = 0;
+#pragma unroll 1
+        for (int sh = 21, bits = 11; bits > 0; bits = sh ? (sh == 10 ? 10 : 11) : 0, sh = sh == 21 ? 10 : 0) {
+            const int bins = 1 << bits;
+            for (int i = tid; i < bins; i += kEvThreads) s_hist[i] = 0;
             __syncthreads();
-            for (int j = b0 + tid; j < b1; j += kEvThreads) {
-                const uint32_t key = weight_key(w[j]);
-                if (pass == 0 || (key >> (sh + bits[pass])) == prefix) atomicAdd(&hist[(key >> sh) & (bins - 1)], 1u);
+#pragma unroll 2
+            for (int base = 0; base < len; base += kEvThreads) {
+                const uint32_t key = key_at(base + tid);
+                const bool in = base + tid < len && (sh == 21 || key >> (sh + bits) == t);
+                const uint32_t digit = key >> sh & (bins - 1);
+                // many equal weights (a fresh cache's zeros) would all meet in one bin: one lane
+                // adds for those that share the first one's digit
+                const uint32_t who = __ballot_sync(0xffffffffu, in);
+                const int first = who ? __ffs(who) - 1 : 0;
+                const uint32_t lead = __shfl_sync(0xffffffffu, digit, first);
+                const uint32_t same = __ballot_sync(0xffffffffu, in && digit == lead);
+                if (in && lane == first) atomicAdd(&s_hist[digit], (uint32_t)__popc(same));
+                else if (in && digit != lead) atomicAdd(&s_hist[digit], 1u);
             }
-            cl.sync();
-            // bins from the top, a run of them per thread
-            const int run = bins / kEvThreads;
-            uint32_t c[kEvBins / kEvThreads];
-            int mine = 0;
+            if (parts > 1) cl.sync();
+            else __syncthreads();
+            // bins from the top, a run of them per thread; the one in which the left-th
+            // largest key lies
+            const int run = bins / kEvThreads, top = bins - 1 - tid * run;
+            int cnt[kEvBins / kEvThreads], mine = 0;
 #pragma unroll
             for (int i = 0; i < kEvBins / kEvThreads; ++i) {
-                c[i] = 0;
+                cnt[i] = 0;
                 if (i < run) {
-                    const int b = bins - 1 - (tid * run + i);
-#pragma unroll
-                    for (int r = 0; r < kEvC; ++r) c[i] += cl.map_shared_rank(hist, r)[b];
-                    mine += (int)c[i];
+                    if (parts == 1) cnt[i] = (int)s_hist[top - i];
+                    else
+                        for (int r = 0; r < parts; ++r) cnt[i] += (int)cl.map_shared_rank(s_hist, r)[top - i];
                 }
+                mine += cnt[i];
             }
-            int total;
-            int before = block_excl(mine, s_warp, &total);
-            // the bin in which the left-th largest key lies (left == 0: no key is kept)
+            int before = block_excl(mine, s_warp);
+            if (before < left && before + mine >= left) {
+                int i = 0;
 #pragma unroll
-            for (int i = 0; i < kEvBins / kEvThreads; ++i) {
-                if (i < run) {
-                    if (before < left && before + (int)c[i] >= left)
-                        s_digit = bins - 1 - (tid * run + i), s_above = before;
-                    before += (int)c[i];
-                }
+                for (int q = 0; q < kEvBins / kEvThreads - 1; ++q)
+                    if (i == q && before + cnt[q] < left) before += cnt[q], ++i;
+                s_tot[0] = top - i, s_tot[1] = before;
             }
-            if (left == 0 && tid == 0) s_digit = bins - 1, s_above = 0;
-            __syncthreads();
-            prefix = (prefix << bits[pass]) | s_digit;
-            left -= (int)s_above;
+            if (parts > 1) cl.sync();  // (also: the histograms have been read)
+            else __syncthreads();
+            t = t << bits | (uint32_t)s_tot[0];
+            left -= s_tot[1];
             __syncthreads();
         }
         // above the threshold: kept; equal to it: the first `left` of them
-        int ngt = 0, neq = 0;
-        for (int j = b0 + tid; j < b1; j += kEvThreads) {
-            const uint32_t key = weight_key(w[j]);
-            ngt += key > prefix, neq += key == prefix;
+        int gt0 = 0, eq0 = 0;  // in the CTAs and the chunks before
+        if (parts > 1) {
+            int g = 0, q = 0;
+            for (int j = tid; j < len; j += kEvThreads) {
+                const uint32_t key = key_at(j);
+                g += key > t, q += key == t;
+            }
+            const int pg = block_excl(g, s_warp), pq = block_excl(q, s_warp);
+            if (tid == kEvThreads - 1) s_tot[0] = pg + g, s_tot[1] = pq + q;
+            cl.sync();
+            gt0 = __reduce_add_sync(0xffffffffu, lane < rank ? cl.map_shared_rank(s_tot, lane)[0] : 0);
+            eq0 = __reduce_add_sync(0xffffffffu, lane < rank ? cl.map_shared_rank(s_tot, lane)[1] : 0);
+            cl.sync();
         }
-        if (need == 0) ngt = 0;
-        int tgt, teq;
-        block_excl(ngt, s_warp, &tgt);
-        block_excl(neq, s_warp, &teq);
-        if (tid == 0) s_cnt[0] = tgt, s_cnt[1] = teq;
-        cl.sync();
-        int gt0 = 0, eq0 = 0;
-        for (int r = 0; r < rank; ++r) {
-            const int* c = cl.map_shared_rank(s_cnt, r);
-            gt0 += c[0], eq0 += c[1];
-        }
-        for (int j = rank * kEvThreads + tid; j < e.n_sink; j += kEvC * kEvThreads) kept[j] = j;
-        for (int j = rank * kEvThreads + tid; j < e.n_recent; j += kEvC * kEvThreads)
-            kept[e.budget - e.n_recent + j] = n - e.n_recent + j;
-        for (int base = b0; base < b1 && need > 0; base += kEvThreads) {
-            const int j = base + tid;
-            const uint32_t key = j < b1 ? weight_key(w[j]) : 0u;
-            const bool gt = j < b1 && key > prefix, eq = j < b1 && key == prefix;
-            int ng, ne;
-            const int g = gt0 + block_excl(gt, s_warp, &ng);
-            const int q = eq0 + block_excl(eq, s_warp, &ne);
-            if (gt || (eq && q < left)) kept[e.n_sink + g + min(q, left)] = j;
-            gt0 += ng, eq0 += ne;
+#pragma unroll 1
+        for (int c0 = 0; c0 < len; c0 += kEvChunk) {
+            const int rows = min(kEvRows, (len - c0 + kEvThreads - 1) / kEvThreads);  // of kEvThreads positions
+#pragma unroll 1
+            for (int i = 0; i < kEvRows; ++i) {
+                const int j = c0 + i * kEvThreads + tid;
+                const uint32_t key = key_at(j);
+                const uint32_t bg = __ballot_sync(0xffffffffu, j < len && key > t), bq = __ballot_sync(0xffffffffu, j < len && key == t);
+                if (lane == 0) s_at[0][i * kEvWarps + warp] = __popc(bg), s_at[1][i * kEvWarps + warp] = __popc(bq);
+            }
+            __syncthreads();
+            // exclusive sums in the order of the positions, both kinds at once: 256 each
+            {
+                const int kind = tid >> 8, at = tid & 255, v = s_at[kind][at];
+                const int x = block_excl(v, s_warp);
+                if (tid == 255) s_tot[0] = x + v;
+                __syncthreads();
+                if (tid == kEvThreads - 1) s_tot[1] = x + v - s_tot[0];
+                s_at[kind][at] = x - (kind ? s_tot[0] : 0);
+            }
+            __syncthreads();
+            const uint32_t below = (1u << lane) - 1u;
+#pragma unroll 1
+            for (int i = 0; i < rows; ++i) {
+                const int j = c0 + i * kEvThreads + tid;
+                const uint32_t key = key_at(j);
+                const bool g = j < len && key > t, q = j < len && key == t;
+                const uint32_t bg = __ballot_sync(0xffffffffu, g), bq = __ballot_sync(0xffffffffu, q);
+                const int pg = gt0 + s_at[0][i * kEvWarps + warp] + __popc(bg & below);
+                const int pq = eq0 + s_at[1][i * kEvWarps + warp] + __popc(bq & below);
+                if (g || (q && pq < left)) kept[e.n_sink + pg + min(pq, left)] = b0 + j;
+            }
+            gt0 += s_tot[0], eq0 += s_tot[1];
+            __syncthreads();  // the counts are written again by the next chunk
         }
     }
-    cl.sync();  // kept is complete (and no CTA reads another's shared memory any more)
+    cl.sync();  // no CTA ends while another may read its shared memory
+}
 
-    // ---- move
-    const int pieces = a.hd / 8;                 // 16-byte pieces of one row of K (or V)
-    const int per_row = 2 * pieces;
-    const int rows_cta = kEvThreads / per_row;   // rows of one register step of a CTA
-    const int lr = tid / per_row, c = tid - lr * per_row;
-    const bool isv = c >= pieces;
-    const int piece = (isv ? c - pieces : c) * 8;
-    constexpr int U = 4;
-    const int step = kEvC * rows_cta * U;
-    const float* wsrc = w;
-    float* wdst = e.w_dst ? e.w_dst + row * e.w_stride : nullptr;
-    for (int c0 = 0; c0 < m; c0 += step) {
-        uint4 x[U];
-        int64_t to[U];
-        float wv[U];
+// ---- move, to pages that the source does not hold: one warp (or two half ones) per
+// kept row, a 16-byte piece of K or V per lane, kMoveU rows each; enough in flight
+// for the memory's rate.  The weights move along, the rest of their row is cleared.
+constexpr int kMoveU = 4, kMoveThreads = 256;
+
+__global__ void __launch_bounds__(kMoveThreads) k_paged_move(EvictArgs e) {
+    pdl_begin();
+    const PagedArgs& a = e.src;
+    const int h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x;
+    const int n = seq_len(a, s), m = n < e.budget ? n : e.budget;
+    const int64_t row = (int64_t)s * a.nkv + h;
+    const int32_t* kept = e.kept + row * e.budget;
+    const int pieces = a.hd / 8, per_row = 2 * pieces, rows_cta = kMoveThreads / per_row;
+    const int lr = tid / per_row, c = tid - lr * per_row, piece = (c >= pieces ? c - pieces : c) * 8;
+    const uint16_t* from = c >= pieces ? a.v : a.k;
+    uint16_t* to = const_cast<uint16_t*>(c >= pieces ? e.dst.v : e.dst.k);
+    const int j0 = blockIdx.x * (rows_cta * kMoveU);
+    if (lr < rows_cta) {
+        int64_t src[kMoveU], dst[kMoveU];
+        uint4 x[kMoveU];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+        for (int u = 0; u < kMoveU; ++u) {
+            const int j = j0 + u * rows_cta + lr;
+            src[u] = dst[u] = -1;
+            if (j < m) src[u] = row_offset(a, s, kept[j], h), dst[u] = row_offset(e.dst, s, j, h);
+        }
+#pragma unroll
+        for (int u = 0; u < kMoveU; ++u)
+            if (src[u] >= 0) x[u] = *reinterpret_cast<const uint4*>(from + src[u] + piece);
+#pragma unroll
+        for (int u = 0; u < kMoveU; ++u)
+            if (src[u] >= 0 && dst[u] >= 0) *reinterpret_cast<uint4*>(to + dst[u] + piece) = x[u];
+    }
+    if (!e.w_dst) return;
+    const float* w = e.w + row * e.w_stride;
+    float* wd = e.w_dst + row * e.w_stride;
+    for (int j = blockIdx.x * kMoveThreads + tid; j < e.w_stride; j += gridDim.x * kMoveThreads) wd[j] = j < m ? w[kept[j]] : 0.0f;
+}
+
+// ---- move in place: places [c0, c1) come from positions >= c0, so with a cluster
+// barrier between a step's reads and its writes a later step finds its rows (at
+// positions >= c1) as they were
+__global__ void __cluster_dims__(kEvC, 1, 1) __launch_bounds__(kEvThreads, 2) k_paged_move_in_place(EvictArgs e) {
+    pdl_begin();
+    cg::cluster_group cl = cg::this_cluster();
+    const PagedArgs& a = e.src;
+    const int rank = (int)cl.block_rank(), h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x;
+    const int n = seq_len(a, s), m = n < e.budget ? n : e.budget;
+    const int64_t row = (int64_t)s * a.nkv + h;
+    const int32_t* kept = e.kept + row * e.budget;
+    const float* w = e.w + row * e.w_stride;
+    float* wd = e.w_dst ? e.w_dst + row * e.w_stride : nullptr;
+    const int pieces = a.hd / 8, per_row = 2 * pieces, rows_cta = kEvThreads / per_row;
+    const int lr = tid / per_row, c = tid - lr * per_row, piece = (c >= pieces ? c - pieces : c) * 8;
+    const uint16_t* from = c >= pieces ? a.v : a.k;
+    uint16_t* to = const_cast<uint16_t*>(c >= pieces ? e.dst.v : e.dst.k);
+    const int step = kEvC * rows_cta * kMoveU;
+    for (int c0 = 0; c0 < m; c0 += step) {
+        int64_t dst[kMoveU];
+        uint4 x[kMoveU];
+        float wv[kMoveU];
+#pragma unroll
+        for (int u = 0; u < kMoveU; ++u) {
             const int j = c0 + (u * kEvC + rank) * rows_cta + lr;
-            to[u] = -1;
+            dst[u] = -1, wv[u] = 0.0f;
             if (lr < rows_cta && j < m) {
-                const int from = kept[j];
-                if (c == 0) wv[u] = wsrc[from];
-                const int64_t src = row_offset(a, s, from, h);
-                to[u] = row_offset(e.dst, s, j, h);
-                if (src < 0) to[u] = -1;
-                if (to[u] >= 0) x[u] = *reinterpret_cast<const uint4*>((isv ? a.v : a.k) + src + piece);
+                const int i = kept[j];
+                const int64_t src = row_offset(a, s, i, h);
+                if (c == 0) wv[u] = w[i];
+                if (src >= 0) dst[u] = row_offset(e.dst, s, j, h), x[u] = *reinterpret_cast<const uint4*>(from + src + piece);
             }
         }
-        if (e.in_place) cl.sync();
+        cl.sync();
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+        for (int u = 0; u < kMoveU; ++u) {
             const int j = c0 + (u * kEvC + rank) * rows_cta + lr;
-            if (to[u] >= 0) {
-                *reinterpret_cast<uint4*>(const_cast<uint16_t*>(isv ? e.dst.v : e.dst.k) + to[u] + piece) = x[u];
-            }
-            if (wdst && lr < rows_cta && j < m && c == 0) wdst[j] = wv[u];
+            if (dst[u] >= 0) *reinterpret_cast<uint4*>(to + dst[u] + piece) = x[u];
+            if (wd && lr < rows_cta && j < m && c == 0) wd[j] = wv[u];
         }
     }
-    // the rest of the weights' row is cleared for the positions to come
-    if (e.in_place) cl.sync();
-    if (wdst)
-        for (int j = m + rank * kEvThreads + tid; j < e.w_stride; j += kEvC * kEvThreads) wdst[j] = 0.0f;
+    cl.sync();
+    if (wd)
+        for (int j = m + rank * kEvThreads + tid; j < e.w_stride; j += kEvC * kEvThreads) wd[j] = 0.0f;
 }
 
 // ------------------------------------------------- attention, the plain kernel
@@ -308,7 +380,16 @@ cudaError_t launch_paged_evict(const PagedArgs& src, const PagedArgs& dst, const
                                int budget, int n_sink, int n_recent, int32_t* kept, int32_t* new_len, cudaStream_t st) {
     EvictArgs e{src, dst, w, w_dst, w_stride, budget, n_sink, n_recent, kept, new_len,
                 src.k == dst.k || src.v == dst.v || w == w_dst};
-    const cudaError_t r = launch_pdl(k_paged_evict, dim3(kEvC, src.nkv, src.n_seqs), dim3(kEvThreads), 0, st, e);
+    // more positions than one CTA holds: a cluster for each (sequence, KV head)
+    const int size = src.cap > kEvChunk ? kEvC : 1;
+    cudaError_t r = launch_pdl_cluster(k_paged_select, dim3(size, src.nkv, src.n_seqs), dim3(kEvThreads), size, st, e);
+    if (r != cudaSuccess) return r;
+    if (e.in_place) {
+        r = launch_pdl(k_paged_move_in_place, dim3(kEvC, src.nkv, src.n_seqs), dim3(kEvThreads), 0, st, e);
+    } else {
+        const int rows = kMoveThreads / (src.hd / 4) * kMoveU, most = budget < src.cap ? budget : src.cap;
+        r = launch_pdl(k_paged_move, dim3((most + rows - 1) / rows, src.nkv, src.n_seqs), dim3(kMoveThreads), 0, st, e);
+    }
     return r != cudaSuccess ? r : cudaGetLastError();
 }
 
