@@ -38,7 +38,8 @@ namespace {
 constexpr int kTile = 64;                       // positions per tile: 16 per warp
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kStages = 3;                      // per warp
-constexpr int kMaxParts = 128;                  // parts whose factors are held at once
+constexpr int kMinTiles = 3;                    // of a CTA's run: fewer parts to join (one sequence of 2049: 9.3 us,
+                                                // with 1 or 2 tiles 9.9 and 10.1, with 4 or 6 11.2 and 12.6)
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -121,8 +122,7 @@ struct DecodeSmem {
     static constexpr int RING = kWarps * kStages * STAGE;
     static constexpr int MRG_LD = 64 + 4;                    // a head's row in the joining buffer
     static constexpr int MRG = kWarps * 8 * MRG_LD * 4;      // one half of the dimensions of 8 heads
-    static constexpr int W = kMaxParts * kPagedMaxGroup * 4; // factors of the parts
-    static constexpr int BYTES = RING + (MRG > W ? MRG : W);
+    static constexpr int BYTES = RING + MRG;
 };
 
 template <int DT, int HD, int NT>
@@ -133,61 +133,90 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     float* s_mrg = reinterpret_cast<float*>(smem + M::RING);
     __shared__ float s_m[kWarps][16], s_l[kWarps][16];
-    __shared__ float s_M[16], s_L[16];
-    __shared__ long long s_scan[kWarps];
-    __shared__ long long s_first;
+    __shared__ uint32_t s_scan[kWarps], s_first;
     __shared__ int s_seq;
     __shared__ int s_last;
     const PagedArgs& a = p.c;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int nq = a.nkv * a.group, G = a.group;
 
-    // ---- this CTA's run of the line
-    const int per = (a.n_seqs + kThreads - 1) / kThreads;
-    const int sb = min(a.n_seqs, tid * per), se = min(a.n_seqs, sb + per);
-    long long mine = 0;
-    for (int s = sb; s < se; ++s) mine += span_of(seq_len(a, s), p.window, p.n_sink).nt;
-    long long incl = mine;
+    // ---- this CTA's run of the line: N tiles in `grid` runs, the first `more` of them
+    // one longer than the others
+    uint32_t N, first = 0;
+    int seq = 0;
+    auto cut = [&](uint32_t total, uint32_t* grid, uint32_t* each, uint32_t* more) {
+        *grid = min((uint32_t)gridDim.x, max(1u, total / kMinTiles));
+        *each = total / *grid, *more = total - *each * *grid;
+    };
+    uint32_t grid, each, more, u0;
+    auto start_of = [&](uint32_t c) { return c * each + min(c, more); };
+    auto owner_of = [&](uint32_t u) {
+        const uint32_t longer = more * (each + 1);
+        return u < longer ? u / (each + 1) : more + (u - longer) / each;
+    };
+    if (a.n_seqs <= 32) {
+        // every warp for itself, a sequence per lane
+        const uint32_t mine = lane < a.n_seqs ? span_of(seq_len(a, lane), p.window, p.n_sink).nt * a.nkv : 0;
+        uint32_t incl = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
-    }
-    if (lane == 31) s_scan[warp] = incl;
-    __syncthreads();
-    long long total = 0, before = incl - mine;
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        N = __shfl_sync(0xffffffffu, incl, 31);
+        cut(N, &grid, &each, &more);
+        u0 = start_of(min((uint32_t)blockIdx.x, grid));
+        const uint32_t who = __ballot_sync(0xffffffffu, u0 >= incl - mine && u0 < incl);
+        seq = who ? __ffs(who) - 1 : 0;
+        first = __shfl_sync(0xffffffffu, incl - mine, seq);
+    } else {
+        const int per = (a.n_seqs + kThreads - 1) / kThreads;
+        const int sb = min(a.n_seqs, tid * per), se = min(a.n_seqs, sb + per);
+        uint32_t mine = 0;
+        for (int s = sb; s < se; ++s) mine += span_of(seq_len(a, s), p.window, p.n_sink).nt * a.nkv;
+        uint32_t incl = mine;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += s_scan[w];
-        total += s_scan[w];
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        if (lane == 31) s_scan[warp] = incl;
+        __syncthreads();
+        uint32_t before = incl - mine;
+        N = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) before += s_scan[w];
+            N += s_scan[w];
+        }
+        cut(N, &grid, &each, &more);
+        u0 = start_of(min((uint32_t)blockIdx.x, grid));
+        if (u0 >= before && u0 < before + mine) {
+            uint32_t b = before;
+            for (int s = sb; s < se; ++s) {
+                const uint32_t c = span_of(seq_len(a, s), p.window, p.n_sink).nt * a.nkv;
+                if (u0 < b + c) {
+                    s_seq = s, s_first = b;
+                    break;
+                }
+                b += c;
+            }
+        }
+        __syncthreads();
+        seq = s_seq, first = s_first;
     }
-    const long long N = total * a.nkv;
-    const long long grid = N < (long long)gridDim.x ? N : (long long)gridDim.x;
     // a sequence without positions gives zeros
     for (int s = blockIdx.x; s < a.n_seqs; s += gridDim.x)
         if (seq_len(a, s) == 0)
             for (int i = tid; i < nq * a.hd; i += kThreads) p.out[(int64_t)s * nq * a.hd + i] = 0;
-    if ((long long)blockIdx.x >= grid) return;
-    const long long u0 = N * blockIdx.x / grid, u1 = N * (blockIdx.x + 1) / grid;
-    {
-        long long b = before * a.nkv;
-        for (int s = sb; s < se; ++s) {
-            const long long c = (long long)span_of(seq_len(a, s), p.window, p.n_sink).nt * a.nkv;
-            if (u0 >= b && u0 < b + c) s_seq = s, s_first = b;
-            b += c;
-        }
-    }
-    __syncthreads();
+    if (blockIdx.x >= grid || N == 0) return;
+    const int count = (int)(start_of(blockIdx.x + 1) - u0);
     Place ld;
-    ld.s = s_seq;
-    ld.sp = span_of(seq_len(a, ld.s), p.window, p.n_sink);
-    {
-        const long long r = u0 - s_first;
-        ld.h = (int)(r / ld.sp.nt);
-        ld.x = (int)(r - (long long)ld.h * ld.sp.nt);
-    }
+    ld.s = seq;
+    ld.sp = span_of(seq_len(a, seq), p.window, p.n_sink);
+    ld.h = (int)((u0 - first) / (uint32_t)ld.sp.nt);
+    ld.x = (int)(u0 - first) - ld.h * ld.sp.nt;
     Place cs = ld;  // the consumer's place; ld runs ahead
-    const int count = (int)(u1 - u0);
 
     // ---- loads: this warp's 16 rows of the tile at `ld` into stage st
     const uint32_t ring = smem_u32(smem) + warp * (kStages * M::STAGE);
@@ -214,7 +243,24 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
             cp16(dst + M::HALF, a.v + src, take);
         }
     };
+    // B fragments of q: head 8 nt + g, dimensions 16 kk + 2t, + 8
+    uint32_t qf[NT][HD / 16][2];
+    auto load_q = [&]() {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int head = nt * 8 + g;
+            const uint16_t* q = p.q + cs.s * p.q_stride + (cs.h * G + head) * a.hd;
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const int d = 16 * kk + 8 * b + 2 * t;
+                    qf[nt][kk][b] = head < G && d < a.hd ? *reinterpret_cast<const uint32_t*>(q + d) : 0u;
+                }
+        }
+    };
     int64_t off = lookup(ld);
+    load_q();
     int loaded = 0;  // tiles issued
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) {
@@ -226,7 +272,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
     }
 
     // ---- the loop
-    uint32_t qf[NT][HD / 16][2];
     float acc[NT][HD / 16][4], m[NT][2], l[NT][2];
     bool fresh = true;
     int x_first = 0;
@@ -234,18 +279,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
         if (fresh) {
             fresh = false;
             x_first = cs.x;
-            // B fragments of q: head 8 nt + g, dimensions 16 kk + 2t, + 8
+            if (u) load_q();
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const int head = nt * 8 + g;
-                const uint16_t* q = p.q + cs.s * p.q_stride + (cs.h * G + head) * a.hd;
-#pragma unroll
-                for (int kk = 0; kk < HD / 16; ++kk)
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const int d = 16 * kk + 8 * b + 2 * t;
-                        qf[nt][kk][b] = head < G && d < a.hd ? *reinterpret_cast<const uint32_t*>(q + d) : 0u;
-                    }
 #pragma unroll
                 for (int i = 0; i < HD / 16; ++i)
 #pragma unroll
@@ -285,10 +321,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
                 const int j = j0 + (e >> 1) * 8;
                 const bool vis = j < cs.sp.n && (j < cs.sp.sink_end || j >= cs.sp.lo);
                 x[e] = vis ? s[nt][e] * p.scale_log2 : -INFINITY;
-                if (p.scores && vis) {
-                    const int head = nt * 8 + 2 * t + (e & 1);
-                    if (head < G) p.scores[((int64_t)cs.s * nq + cs.h * G + head) * p.score_ld + j] = x[e];
-                }
+            }
+            if (p.scores && nt * 8 + 2 * t < p.score_heads) {
+                // [j][head of the group]: a warp's store is one run
+                float* sc = p.scores + (((int64_t)cs.s * a.nkv + cs.h) * p.score_ld + j0) * p.score_heads + nt * 8 + 2 * t;
+                if (j0 < cs.sp.n) *reinterpret_cast<float2*>(sc) = make_float2(x[0], x[1]);
+                if (j0 + 8 < cs.sp.n) *reinterpret_cast<float2*>(sc + 8 * p.score_heads) = make_float2(x[2], x[3]);
             }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {  // head 2t + c of the eight
@@ -333,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
         }
         // ---- the end of a run of (s, h): the four warps' parts at a common maximum
         const bool whole = item_end && x_first == 0;
-        const long long first_u = u0 + u - cs.x, last_u = first_u + cs.sp.nt - 1;
+        const uint32_t first_u = u0 + u - cs.x, last_u = first_u + cs.sp.nt - 1;
         const int slot = 2 * blockIdx.x + (x_first == 0 ? 1 : 0);
         float* part = p.part + (int64_t)slot * part_floats(G, HD);
 #pragma unroll
@@ -396,58 +434,59 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
         }
         if (!whole) {
             // ---- the last CTA of the item joins its parts, in their order
-            const int c0 = (int)(((first_u + 1) * grid - 1) / N), c1 = (int)(((last_u + 1) * grid - 1) / N);
+            const int c0 = (int)owner_of(first_u), c1 = (int)owner_of(last_u);
             const int parts = c1 - c0 + 1;
-            __threadfence();
             __syncthreads();
-            if (tid == 0) s_last = atomicInc(p.count + c0, parts - 1) == (unsigned)(parts - 1);
+            if (tid == 0) {
+                __threadfence();
+                s_last = atomicInc(p.count + c0, parts - 1) == (unsigned)(parts - 1);
+            }
             __syncthreads();
             if (s_last) {
                 __threadfence();
-                auto base = [&](int i) { return p.part + (int64_t)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * part_floats(G, HD); };
-                for (int head = warp; head < G; head += kWarps) {
-                    float mx = -INFINITY, ls = 0.0f;
-                    for (int i = lane; i < parts; i += 32)
-                        mx = fmaxf(mx, __ldcg(reinterpret_cast<const float2*>(base(i) + G * HD) + head).x);
+                constexpr int V4 = HD / 4;                                  // float4 per head
+                constexpr int PER = (NT * 8 * V4 + kThreads - 1) / kThreads;  // of each thread
+                constexpr int B = 8 / NT;                                   // parts in flight
+                const int pf = part_floats(G, HD);
+                float o[PER][4], M[PER], L[PER];
 #pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                    const float ref = mx == -INFINITY ? 0.0f : mx;
-                    for (int i = lane; i < parts; i += 32) {
-                        const float2 v = __ldcg(reinterpret_cast<const float2*>(base(i) + G * HD) + head);
-                        ls += ex2(v.x - ref) * v.y;
-                    }
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, o);
-                    if (lane == 0) {
-                        s_M[head] = ref, s_L[head] = ls;
-                        if (p.ml) p.ml[(int64_t)cs.s * nq + cs.h * G + head] = make_float2(ref, ls);
-                    }
-                }
-                constexpr int V4 = HD / 4;
-                constexpr int PER = (NT * 8 * V4 + kThreads - 1) / kThreads;
-                float o[PER][4];
-#pragma unroll
-                for (int r = 0; r < PER; ++r)
+                for (int r = 0; r < PER; ++r) {
+                    M[r] = -INFINITY, L[r] = 0.0f;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[r][e] = 0.0f;
-                for (int p0 = 0; p0 < parts; p0 += kMaxParts) {
-                    const int np = min(kMaxParts, parts - p0);
-                    __syncthreads();
-                    for (int i = tid; i < np * G; i += kThreads) {
-                        const int pi = i / G, head = i - pi * G;
-                        s_mrg[pi * G + head] =
-                            ex2(__ldcg(reinterpret_cast<const float2*>(base(p0 + pi) + G * HD) + head).x - s_M[head]);
+                }
+                for (int p0 = 0; p0 < parts; p0 += B) {
+                    float4 x[PER][B];
+                    float2 ml[PER][B];
+#pragma unroll
+                    for (int k = 0; k < B; ++k) {
+                        const int i = p0 + k;
+                        const float* base = p.part + (int64_t)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * pf;
+#pragma unroll
+                        for (int r = 0; r < PER; ++r) {
+                            const int v = r * kThreads + tid, head = v / V4;
+                            ml[r][k] = make_float2(-INFINITY, 0.0f), x[r][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            if (i < parts && head < G) {
+                                ml[r][k] = __ldcg(reinterpret_cast<const float2*>(base + G * HD) + head);
+                                x[r][k] = __ldcg(reinterpret_cast<const float4*>(base) + v);
+                            }
+                        }
                     }
-                    __syncthreads();
 #pragma unroll
                     for (int r = 0; r < PER; ++r) {
-                        const int v = r * kThreads + tid, head = v / V4;
-                        if (head >= G) continue;
-#pragma unroll 8
-                        for (int pi = 0; pi < np; ++pi) {
-                            const float4 x = __ldcg(reinterpret_cast<const float4*>(base(p0 + pi)) + v);
-                            const float f = s_mrg[pi * G + head];
-                            o[r][0] += f * x.x, o[r][1] += f * x.y, o[r][2] += f * x.z, o[r][3] += f * x.w;
+                        float mx = M[r];
+#pragma unroll
+                        for (int k = 0; k < B; ++k) mx = fmaxf(mx, ml[r][k].x);
+                        const float ref = mx == -INFINITY ? 0.0f : mx, old = ex2(M[r] - ref);
+                        M[r] = mx, L[r] *= old;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[r][e] *= old;
+#pragma unroll
+                        for (int k = 0; k < B; ++k) {
+                            const float f = ex2(ml[r][k].x - ref);
+                            L[r] += f * ml[r][k].y;
+                            o[r][0] += f * x[r][k].x, o[r][1] += f * x[r][k].y;
+                            o[r][2] += f * x[r][k].z, o[r][3] += f * x[r][k].w;
                         }
                     }
                 }
@@ -455,10 +494,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
                 for (int r = 0; r < PER; ++r) {
                     const int v = r * kThreads + tid, head = v / V4, d = (v - head * V4) * 4;
                     if (head < G && d < a.hd) {
-                        const float ls = s_L[head];
                         uint16_t* dst = p.out + ((int64_t)cs.s * nq + cs.h * G + head) * a.hd + d;
-                        *reinterpret_cast<uint2*>(dst) =
-                            make_uint2(X::pack(o[r][0] / ls, o[r][1] / ls), X::pack(o[r][2] / ls, o[r][3] / ls));
+                        *reinterpret_cast<uint2*>(dst) = make_uint2(X::pack(o[r][0] / L[r], o[r][1] / L[r]),
+                                                                    X::pack(o[r][2] / L[r], o[r][3] / L[r]));
+                        if (p.ml && d == 0)
+                            p.ml[(int64_t)cs.s * nq + cs.h * G + head] = make_float2(M[r] == -INFINITY ? 0.0f : M[r], L[r]);
                     }
                 }
             }
@@ -470,22 +510,34 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// weights[s][h][j] += sum over the group of 2^(x_j - M) / L, from the decode's scores.
+// weights[s][h][j] += sum over the group of 2^(x_j - M) / L, from the decode's scores:
+// one position per thread, its scores side by side.
 __global__ void __launch_bounds__(256) k_paged_add_weights(DecodeArgs p) {
     pdl_begin();
+    __shared__ float2 s_ml[kPagedMaxGroup];
     const PagedArgs& a = p.c;
     const int h = blockIdx.y, s = blockIdx.z, nq = a.nkv * a.group;
     const Span sp = span_of(seq_len(a, s), p.window, p.n_sink);
+    if ((int)threadIdx.x < kPagedMaxGroup) {
+        float2 ml = make_float2(0.0f, 0.0f);
+        if ((int)threadIdx.x < a.group) ml = p.ml[(int64_t)s * nq + h * a.group + threadIdx.x], ml.y = 1.0f / ml.y;
+        s_ml[threadIdx.x] = ml;
+    }
+    __syncthreads();
     float* w = p.weights + ((int64_t)s * a.nkv + h) * p.w_stride;
+    const float* sc = p.scores + ((int64_t)s * a.nkv + h) * p.score_ld * p.score_heads;
     for (int j = blockIdx.x * blockDim.x + threadIdx.x; j < sp.n; j += gridDim.x * blockDim.x) {
         if (j >= sp.sink_end && j < sp.lo) continue;
         float sum = 0.0f;
-        for (int g = 0; g < a.group; ++g) {
-            const int64_t row = (int64_t)s * nq + h * a.group + g;
-            const float2 ml = p.ml[row];
-            sum += ex2(p.scores[row * p.score_ld + j] - ml.x) / ml.y;
-        }
-        w[j] += sum;
+        const float old = w[j];
+#pragma unroll
+        for (int g = 0; g < kPagedMaxGroup; g += 2)
+            if (g < p.score_heads) {
+                const float2 x = *reinterpret_cast<const float2*>(sc + (int64_t)j * p.score_heads + g);
+                sum += ex2(x.x - s_ml[g].x) * s_ml[g].y;
+                if (g + 1 < a.group) sum += ex2(x.y - s_ml[g + 1].x) * s_ml[g + 1].y;
+            }
+        w[j] = old + sum;
     }
 }
 
@@ -508,6 +560,7 @@ size_t paged_decode_part_floats(int group, int num_sms) {
 cudaError_t launch_paged_decode(const DecodeArgs& p, int dtype, int num_sms, cudaStream_t st) {
     if (p.c.n_seqs <= 0) return cudaSuccess;
     if (p.c.hd > 128 || p.c.hd % 8 || p.c.group > kPagedMaxGroup) return cudaErrorInvalidValue;
+    if ((int64_t)p.c.n_seqs * p.c.nkv * (p.c.cap / kTile + 2) > 0x7fffffff) return cudaErrorInvalidValue;  // tiles are counted in 32 bits
     const int sel = (dtype ? 4 : 0) + (p.c.hd > 64 ? 2 : 0) + (p.c.group > 8 ? 1 : 0);
     cudaError_t e = cudaErrorInvalidValue;
     switch (sel) {

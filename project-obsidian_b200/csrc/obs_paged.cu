@@ -17,7 +17,7 @@ struct PagedState {
     uint8_t* mem = nullptr;
     float* part = nullptr;      // parts of items that several CTAs share
     uint32_t* count = nullptr;  // their arrivals
-    float* scores = nullptr;    // with cfg.weights: [max_seqs][n_heads][max_kv_len]
+    float* scores = nullptr;    // with cfg.weights: [max_seqs][n_kv_heads][max_kv_len][group, even]
     float* pf_part = nullptr;   // parts of a prefill's rows that several CTAs share
     float2* ml = nullptr;       // with cfg.weights: [max_seqs][n_heads]
 };
@@ -118,7 +118,7 @@ extern "C" int obs_paged_init(obs_ctx* ctx, const obs_paged_config* cfg) {
     ps->cfg = *cfg;
     const size_t n = (size_t)cfg->max_seqs * nq;
     const size_t sizes[] = {paged_decode_part_floats(nq / nkv, parts.num_sms) * 4, (size_t)kPagedCtas * parts.num_sms * 4,
-                            cfg->weights ? n * cfg->max_kv_len * 4 : 0, cfg->weights ? n * 8 : 0,
+                            cfg->weights ? (size_t)cfg->max_seqs * nkv * ((nq / nkv + 1) & ~1) * cfg->max_kv_len * 4 : 0, cfg->weights ? n * 8 : 0,
                             paged_prefill_part_floats(parts.num_sms) * 4};
     void** ptrs[] = {(void**)&ps->part, (void**)&ps->count, (void**)&ps->scores, (void**)&ps->ml, (void**)&ps->pf_part};
     size_t total = 0;
@@ -163,6 +163,8 @@ extern "C" int obs_paged_decode(obs_ctx* ctx, const obs_paged_kv* kv, const void
     PAGED_BEGIN();
     if (a.n_seqs == 0) return OBS_OK;
     if (const char* m = query_args(a, q, q_stride, out, window, n_sink, scale)) return ctx_fail(ctx, OBS_ERR_INVALID, m);
+    if ((int64_t)a.n_seqs * a.nkv * (a.cap / 64 + 2) > 0x7fffffff)
+        return ctx_fail(ctx, OBS_ERR_INVALID, "n_seqs * n_kv_heads * positions is too large for one call");
     if (weights && !ps->cfg.weights)
         return ctx_fail(ctx, OBS_ERR_STATE, "the paged cache was initialised without room for weights");
     if (weights && w_stride <= 0) return ctx_fail(ctx, OBS_ERR_INVALID, "w_stride must be positive");
@@ -170,6 +172,7 @@ extern "C" int obs_paged_decode(obs_ctx* ctx, const obs_paged_kv* kv, const void
     const float sc = scale > 0.0f ? scale : 1.0f / sqrtf((float)a.hd);
     DecodeArgs p{a, reinterpret_cast<const uint16_t*>(q), q_stride, reinterpret_cast<uint16_t*>(out), window, n_sink,
                  sc * kLog2e, ps->part, ps->count, weights ? ps->scores : nullptr, ps->cfg.max_kv_len,
+                 (a.group + 1) & ~1,
                  weights ? ps->ml : nullptr, weights, w_stride};
     return launched(ctx, launch_paged_decode(p, ps->cfg.dtype, parts.num_sms, as_stream(stream)), "paged decode");
 }

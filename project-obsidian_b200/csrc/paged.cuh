@@ -108,8 +108,9 @@ struct DecodeArgs {
     float scale_log2;         // scale * log2(e)
     float* part;              // 2 per CTA: its parts of (sequence, head)s it shares
     uint32_t* count;          // [CTAs] arrivals, zero between launches
-    float* scores;            // with weights: [n_seqs][nq][score_ld] x_j
+    float* scores;            // with weights: [n_seqs][nkv][score_ld][score_heads] x_j
     int64_t score_ld;
+    int score_heads;          // the group, rounded up to even
     float2* ml;               // with weights: [n_seqs][nq] maximum and sum
     float* weights;           // optional: [n_seqs][nkv][w_stride]
     int w_stride;

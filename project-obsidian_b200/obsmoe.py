@@ -118,8 +118,10 @@ class PagedKV:
             raise ValueError("block_table's rows may not overlap")
         self.tensors = (k, v, block_table, kv_len)
         self.dtype, self.kv_shape = k.dtype, tuple(k.shape[1:])  # kv_shape: page_size, n_kv_heads, head_dim
+        self.plan = (*self.kv_shape, "bf16" if "bfloat16" in str(k.dtype) else "f16")
+        self.n_seqs = block_table.shape[0]
         self.view = PagedView(k.data_ptr(), v.data_ptr(), block_table.data_ptr(), kv_len.data_ptr(),
-                              k.stride(0), k.stride(1), k.stride(2), block_table.shape[0], k.shape[0],
+                              k.stride(0), k.stride(1), k.stride(2), self.n_seqs, k.shape[0],
                               block_table.stride(0), block_table.shape[1])
         self.ref = C.byref(self.view)
 
@@ -317,59 +319,68 @@ class MoeContext:
             raise ValueError(f"dtype must be one of {sorted(_DTYPES)}")
         pc = PagedConfig(n_heads, n_kv_heads, head_dim, page_size, max_seqs, max_kv_len, _DTYPES[dtype], int(weights))
         self._chk(lib().obs_paged_init(self._h, C.byref(pc)))
-        self._paged = (page_size, n_kv_heads, head_dim)
-        self._paged_row, self._paged_dtype = n_heads * head_dim, dtype
+        self._paged = (page_size, n_kv_heads, head_dim, dtype)
+        self._paged_row, self._paged_kv_row = n_heads * head_dim, n_kv_heads * head_dim
+
+    _paged = None  # page_size, n_kv_heads, head_dim, dtype after paged_init
 
     def _paged_kv(self, kv):
-        if getattr(self, "_paged", None) is not None:
-            if kv.kv_shape != self._paged:
-                raise ValueError(f"the cache's pages are {kv.kv_shape}, the context's {self._paged}")
-            if ("bf16" if kv.dtype.itemsize == 2 and "bfloat" in str(kv.dtype) else "f16") != self._paged_dtype:
-                raise ValueError(f"the cache holds {kv.dtype}, the context {self._paged_dtype}")
+        if kv.plan != self._paged and self._paged is not None:
+            raise ValueError(f"the cache's pages are {kv.plan}, the context's {self._paged}")
         return kv.ref
 
     def _paged_q(self, kv, q, out, rows):
         """q's row stride, after checks of q and out ([rows, n_heads, head_dim] or [rows, n_heads * head_dim])."""
+        if self._paged is None:  # (the library says what is missing)
+            return 0
         row = self._paged_row
-        if q.dtype != kv.dtype or out.dtype != kv.dtype:
+        if q.dtype is not kv.dtype or out.dtype is not kv.dtype:
             raise ValueError(f"q and out must hold {kv.dtype} like the cache")
         if q.numel() != rows * row or out.numel() != rows * row:
             raise ValueError(f"q and out must be [{rows}, {row}]")
-        if not out.is_contiguous() or (rows and not q[0].is_contiguous()):
-            raise ValueError("out must be consecutive, and each row of q")
+        if not out.is_contiguous():
+            raise ValueError("out must be consecutive")
+        if q.is_contiguous():
+            return row
+        if rows and not q[0].is_contiguous():
+            raise ValueError("each row of q must be consecutive")
         return q.stride(0) if rows > 1 else row
 
     def _paged_w(self, kv, w):
         if w is None:
             return None, 0
-        if w.shape[:2] != (kv.view.n_seqs, kv.kv_shape[1]) or w.element_size() != 4 or not w.is_floating_point() \
-                or not w.is_contiguous():
+        if w.dim() != 3 or w.shape[0] != kv.n_seqs or w.shape[1] != kv.kv_shape[1] or w.element_size() != 4 \
+                or not w.is_floating_point() or not w.is_contiguous():
             raise ValueError("weights: consecutive fp32 [n_seqs, n_kv_heads, positions]")
         return w.data_ptr(), w.shape[2]
 
     def paged_append(self, kv, k, v, seq, slot, T, stream=None):
         """Rows k, v [T, n_kv_heads, head_dim] to positions slot[t] of sequences seq[t]."""
         ref = self._paged_kv(kv)
-        row = self._paged[1] * self._paged[2]
-        if k.dtype != kv.dtype or v.dtype != kv.dtype or k.numel() < T * row or v.numel() < T * row:
+        row = self._paged_kv_row if self._paged else 0
+        if k.dtype is not kv.dtype or v.dtype is not kv.dtype or k.numel() < T * row or v.numel() < T * row:
             raise ValueError(f"k and v must be [T, {row}] of {kv.dtype}")
-        if T and (not k[0].is_contiguous() or not v[0].is_contiguous() or (T > 1 and k.stride(0) != v.stride(0))):
-            raise ValueError("each row of k and v must be consecutive, their strides the same")
-        self._chk(lib().obs_paged_append(self._h, ref, k.data_ptr(), v.data_ptr(), k.stride(0) if T > 1 else row,
-                                         _ptr(seq), _ptr(slot), T, _stream(stream)))
+        stride = row
+        if T and not (k.is_contiguous() and v.is_contiguous()):
+            if not k[0].is_contiguous() or not v[0].is_contiguous() or (T > 1 and k.stride(0) != v.stride(0)):
+                raise ValueError("each row of k and v must be consecutive, their strides the same")
+            stride = k.stride(0) if T > 1 else row
+        self._chk((_LIB or lib()).obs_paged_append(self._h, ref, k.data_ptr(), v.data_ptr(), stride, _ptr(seq),
+                                                   _ptr(slot), T, _stream(stream)))
 
     def paged_decode(self, kv, q, out, window=0, n_sink=0, scale=0.0, weights=None, stream=None):
         """Attention of each sequence's last position over its pages; weights (optional) += the probabilities."""
         ref = self._paged_kv(kv)
         w, ws = self._paged_w(kv, weights)
-        self._chk(lib().obs_paged_decode(self._h, ref, q.data_ptr(), self._paged_q(kv, q, out, kv.view.n_seqs),
-                                         out.data_ptr(), window, n_sink, scale, w, ws, _stream(stream)))
+        self._chk((_LIB or lib()).obs_paged_decode(self._h, ref, q.data_ptr(), self._paged_q(kv, q, out, kv.n_seqs),
+                                                   out.data_ptr(), window, n_sink, scale, w, ws, _stream(stream)))
 
     def paged_prefill(self, kv, q, out, q_start, T, window=0, n_sink=0, scale=0.0, stream=None):
         """Attention of the sequences' last positions, rows q_start[s] .. q_start[s+1] of q each."""
         ref = self._paged_kv(kv)
-        self._chk(lib().obs_paged_prefill(self._h, ref, q.data_ptr(), self._paged_q(kv, q, out, T), out.data_ptr(),
-                                          _ptr(q_start), T, window, n_sink, scale, _stream(stream)))
+        self._chk((_LIB or lib()).obs_paged_prefill(self._h, ref, q.data_ptr(), self._paged_q(kv, q, out, T),
+                                                    out.data_ptr(), _ptr(q_start), T, window, n_sink, scale,
+                                                    _stream(stream)))
 
     def paged_evict(self, kv, dst, weights, weights_dst, budget, n_sink=0, n_recent=0, kept=None, new_len=None,
                     stream=None):
@@ -380,7 +391,7 @@ class MoeContext:
         wd, wds = self._paged_w(kv, weights_dst)
         if wd is not None and wds != ws:
             raise ValueError("weights and weights_dst must have one shape")
-        if kept is not None and kept.numel() < kv.view.n_seqs * kv.kv_shape[1] * budget:
+        if kept is not None and kept.numel() < kv.n_seqs * kv.kv_shape[1] * budget:
             raise ValueError("kept: int32 [n_seqs, n_kv_heads, budget]")
         self._chk(lib().obs_paged_evict(self._h, ref, to, w, wd, ws, budget, n_sink, n_recent, _ptr(kept),
                                         _ptr(new_len), _stream(stream)))
