@@ -682,28 +682,55 @@ __global__ void __launch_bounds__(256) k_paged_join(PrefillArgs p) {
     int s, i;
     if (!find_row(a, p.q_start, t, p.T, &s, &i)) return;
     const int64_t step = (int64_t)p.T * nq;
-    float mx = -INFINITY;
-    for (int z = 0; z < p.splits; ++z) mx = fmaxf(mx, p.part_ml[z * step + row].x);
-    const float ref = mx == -INFINITY ? 0.0f : mx;
-    constexpr int PER = HD / 32;
-    float o[PER] = {}, l = 0.0f;
-#pragma unroll 4
-    for (int z = 0; z < p.splits; ++z) {
-        const float2 ml = p.part_ml[z * step + row];
-        if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // an unused split, or one that saw only -inf
-        const float f = ex2(ml.x - ref);
-        l += f * ml.y;
+    constexpr int PER = HD / 32;  // consecutive dimensions of a lane
+    float M = -INFINITY, o[PER] = {}, l = 0.0f;
+    // 32 splits at a time: a lane reads one split's maximum and sum, then all of them the
+    // split's row
+    for (int z0 = 0; z0 < p.splits; z0 += 32) {
+        const float2 ml = z0 + lane < p.splits ? p.part_ml[(z0 + lane) * step + row] : make_float2(-INFINITY, 0.0f);
+        float mx = ml.x;
 #pragma unroll
-        for (int e = 0; e < PER; ++e) o[e] += f * p.part_acc[(z * step + row) * HD + e * 32 + lane];
+        for (int k = 16; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+        mx = fmaxf(mx, M);
+        const float ref = mx == -INFINITY ? 0.0f : mx, old = ex2(M - ref);
+        M = mx, l *= old;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) o[e] *= old;
+        // (an unused split, or one that saw only -inf, adds nothing: its row may be anything)
+        const bool use = !(ml.x == -INFINITY && ml.y == 0.0f);
+        const float f = use ? ex2(ml.x - ref) : 0.0f;
+        float add = use ? f * ml.y : 0.0f;
+#pragma unroll
+        for (int k = 16; k > 0; k >>= 1) add += __shfl_xor_sync(0xffffffffu, add, k);
+        l += add;
+        const uint32_t used = __ballot_sync(0xffffffffu, use);
+        const float* part = p.part_acc + (z0 * step + row) * HD + lane * PER;
+#pragma unroll 8
+        for (int z = 0; z < min(32, p.splits - z0); ++z) {
+            const float fz = __shfl_sync(0xffffffffu, f, z);
+            if (!(used >> z & 1u)) continue;
+            if constexpr (PER == 4) {
+                const float4 x = *reinterpret_cast<const float4*>(part + z * step * HD);
+                o[0] += fz * x.x, o[1] += fz * x.y, o[2] += fz * x.z, o[3] += fz * x.w;
+            } else {
+                const float2 x = *reinterpret_cast<const float2*>(part + z * step * HD);
+                o[0] += fz * x.x, o[1] += fz * x.y;
+            }
+        }
     }
     bool bad = false;
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-        const int d = e * 32 + lane;
-        const float y = i < 0 ? 0.0f : o[e] / l;
-        bad |= !(fabsf(y) <= 3.4e38f);
-        if (d < a.hd) p.out[row * a.hd + d] = X::h(y);
+        o[e] = i < 0 ? 0.0f : o[e] / l;
+        bad |= !(fabsf(o[e]) <= 3.4e38f);
     }
+    const int d = lane * PER;
+    if (d < a.hd) {
+        uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + row * a.hd + d);
+        if constexpr (PER == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(X::pack(o[0], o[1]), X::pack(o[2], o[3]));
+        else *dst = X::pack(o[0], o[1]);
+    }
+    __syncwarp();
     if (__any_sync(0xffffffffu, bad)) recompute_row<DT>(p, s, head / a.group, t, head, i);
 }
 
