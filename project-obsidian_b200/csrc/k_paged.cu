@@ -47,12 +47,12 @@ __global__ void __launch_bounds__(256) k_paged_append(PagedArgs a, const uint16_
 //            through distributed shared memory.  Ballots then give every kept position
 //            its place, in order.  (Comparing the keys with three candidates a round,
 //            two bits at a time, needs no histogram, but its sixteen rounds took 20 us
-//            where this takes KEEPUS.)
+//            where this takes 5.)
 //   move     the kept rows to places 0, 1, ... of dst.
-constexpr int kEvC = 8, kEvThreads = 512, kEvWarps = kEvThreads / 32;
+constexpr int kEvC = 8, kEvThreads = 1024, kEvWarps = kEvThreads / 32;
 constexpr int kEvBins = 2048;
-constexpr int kEvRows = 16, kEvChunk = kEvRows * kEvThreads;  // positions a CTA holds at a time
-static_assert(2 * kEvRows * kEvWarps == kEvThreads, "one thread per entry of s_at");
+constexpr int kEvRows = 8, kEvChunk = kEvRows * kEvThreads;  // positions a CTA holds at a time
+static_assert(2 * kEvRows * kEvWarps <= kEvThreads, "one thread per entry of s_at");
 
 // larger weight <=> larger key; -0 and +0 equal; NaN the smallest (0)
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -116,8 +116,13 @@ __global__ void __launch_bounds__(kEvThreads) k_paged_select(EvictArgs e) {
         const int per = (hi - lo + parts - 1) / parts;
         const int b0 = min(hi, lo + rank * per), len = min(hi, b0 + per) - b0;
         const bool held = len <= kEvChunk;
-        if (held)
-            for (int j = tid; j < len; j += kEvThreads) s_key[j] = weight_key(w[b0 + j]);  // (each thread reads its own)
+        if (held) {  // (each thread reads its own)
+            float v[kEvRows];
+#pragma unroll
+            for (int i = 0; i < kEvRows; ++i) v[i] = i * kEvThreads + tid < len ? w[b0 + i * kEvThreads + tid] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < kEvRows; ++i) s_key[i * kEvThreads + tid] = weight_key(v[i]);
+        }
         auto key_at = [&](int j) { return j >= len ? 0u : held ? s_key[j] : weight_key(w[b0 + j]); };
         // (the loops are kept rolled: most of this code runs once, and unrolled it was
         // waiting for its instructions)
@@ -135,25 +140,21 @@ __global__ void __launch_bounds__(kEvThreads) k_paged_select(EvictArgs e) {
                 const uint32_t key = key_at(base + tid);
                 const bool in = base + tid < len && (sh == 21 || key >> (sh + bits) == t);
                 const uint32_t digit = key >> sh & (bins - 1);
-                // many equal weights (a fresh cache's zeros) would all meet in one bin: one lane
-                // adds for those that share the first one's digit
-                const uint32_t who = __ballot_sync(0xffffffffu, in);
-                const int first = who ? __ffs(who) - 1 : 0;
-                const uint32_t lead = __shfl_sync(0xffffffffu, digit, first);
-                const uint32_t same = __ballot_sync(0xffffffffu, in && digit == lead);
-                if (in && lane == first) atomicAdd(&s_hist[digit], (uint32_t)__popc(same));
-                else if (in && digit != lead) atomicAdd(&s_hist[digit], 1u);
+                // (equal weights, a fresh cache's zeros, would all meet in one bin: then one lane adds)
+                int one;
+                __match_all_sync(0xffffffffu, in ? digit : 0xffffffffu, &one);
+                if (in && (!one || lane == 0)) atomicAdd(&s_hist[digit], one ? 32u : 1u);
             }
             if (parts > 1) cl.sync();
             else __syncthreads();
             // bins from the top, a run of them per thread; the one in which the left-th
             // largest key lies
-            const int run = bins / kEvThreads, top = bins - 1 - tid * run;
+            const int run = max(1, bins / kEvThreads), top = tid < bins ? bins - 1 - tid * run : -1;
             int cnt[kEvBins / kEvThreads], mine = 0;
 #pragma unroll
             for (int i = 0; i < kEvBins / kEvThreads; ++i) {
                 cnt[i] = 0;
-                if (i < run) {
+                if (i < run && top >= 0) {
                     if (parts == 1) cnt[i] = (int)s_hist[top - i];
                     else
                         for (int r = 0; r < parts; ++r) cnt[i] += (int)cl.map_shared_rank(s_hist, r)[top - i];
@@ -202,12 +203,13 @@ __global__ void __launch_bounds__(kEvThreads) k_paged_select(EvictArgs e) {
             __syncthreads();
             // exclusive sums in the order of the positions, both kinds at once: 256 each
             {
-                const int kind = tid >> 8, at = tid & 255, v = s_at[kind][at];
+                constexpr int kN = kEvRows * kEvWarps;
+                const int kind = tid / kN, at = tid % kN, v = tid < 2 * kN ? s_at[kind][at] : 0;
                 const int x = block_excl(v, s_warp);
-                if (tid == 255) s_tot[0] = x + v;
+                if (tid == kN - 1) s_tot[0] = x + v;
                 __syncthreads();
-                if (tid == kEvThreads - 1) s_tot[1] = x + v - s_tot[0];
-                s_at[kind][at] = x - (kind ? s_tot[0] : 0);
+                if (tid == 2 * kN - 1) s_tot[1] = x + v - s_tot[0];
+                if (tid < 2 * kN) s_at[kind][at] = x - (kind ? s_tot[0] : 0);
             }
             __syncthreads();
             const uint32_t below = (1u << lane) - 1u;
@@ -231,7 +233,7 @@ __global__ void __launch_bounds__(kEvThreads) k_paged_select(EvictArgs e) {
 // ---- move, to pages that the source does not hold: one warp (or two half ones) per
 // kept row, a 16-byte piece of K or V per lane, kMoveU rows each; enough in flight
 // for the memory's rate.  The weights move along, the rest of their row is cleared.
-constexpr int kMoveU = 4, kMoveThreads = 256;
+constexpr int kMoveU = 4, kMoveThreads = 256, kInPlaceThreads = 512;
 
 __global__ void __launch_bounds__(kMoveThreads) k_paged_move(EvictArgs e) {
     pdl_begin();
@@ -270,7 +272,7 @@ __global__ void __launch_bounds__(kMoveThreads) k_paged_move(EvictArgs e) {
 // ---- move in place: places [c0, c1) come from positions >= c0, so with a cluster
 // barrier between a step's reads and its writes a later step finds its rows (at
 // positions >= c1) as they were
-__global__ void __cluster_dims__(kEvC, 1, 1) __launch_bounds__(kEvThreads, 2) k_paged_move_in_place(EvictArgs e) {
+__global__ void __cluster_dims__(kEvC, 1, 1) __launch_bounds__(kInPlaceThreads, 2) k_paged_move_in_place(EvictArgs e) {
     pdl_begin();
     cg::cluster_group cl = cg::this_cluster();
     const PagedArgs& a = e.src;
@@ -280,7 +282,7 @@ __global__ void __cluster_dims__(kEvC, 1, 1) __launch_bounds__(kEvThreads, 2) k_
     const int32_t* kept = e.kept + row * e.budget;
     const float* w = e.w + row * e.w_stride;
     float* wd = e.w_dst ? e.w_dst + row * e.w_stride : nullptr;
-    const int pieces = a.hd / 8, per_row = 2 * pieces, rows_cta = kEvThreads / per_row;
+    const int pieces = a.hd / 8, per_row = 2 * pieces, rows_cta = kInPlaceThreads / per_row;
     const int lr = tid / per_row, c = tid - lr * per_row, piece = (c >= pieces ? c - pieces : c) * 8;
     const uint16_t* from = c >= pieces ? a.v : a.k;
     uint16_t* to = const_cast<uint16_t*>(c >= pieces ? e.dst.v : e.dst.k);
@@ -310,7 +312,7 @@ __global__ void __cluster_dims__(kEvC, 1, 1) __launch_bounds__(kEvThreads, 2) k_
     }
     cl.sync();
     if (wd)
-        for (int j = m + rank * kEvThreads + tid; j < e.w_stride; j += kEvC * kEvThreads) wd[j] = 0.0f;
+        for (int j = m + rank * kInPlaceThreads + tid; j < e.w_stride; j += kEvC * kInPlaceThreads) wd[j] = 0.0f;
 }
 
 // ------------------------------------------------- attention, the plain kernel
@@ -385,7 +387,7 @@ cudaError_t launch_paged_evict(const PagedArgs& src, const PagedArgs& dst, const
     cudaError_t r = launch_pdl_cluster(k_paged_select, dim3(size, src.nkv, src.n_seqs), dim3(kEvThreads), size, st, e);
     if (r != cudaSuccess) return r;
     if (e.in_place) {
-        r = launch_pdl(k_paged_move_in_place, dim3(kEvC, src.nkv, src.n_seqs), dim3(kEvThreads), 0, st, e);
+        r = launch_pdl(k_paged_move_in_place, dim3(kEvC, src.nkv, src.n_seqs), dim3(kInPlaceThreads), 0, st, e);
     } else {
         const int rows = kMoveThreads / (src.hd / 4) * kMoveU, most = budget < src.cap ? budget : src.cap;
         r = launch_pdl(k_paged_move, dim3((most + rows - 1) / rows, src.nkv, src.n_seqs), dim3(kMoveThreads), 0, st, e);
