@@ -11,8 +11,10 @@ namespace obs {
 namespace {
 
 // Row t of k and v ([T] rows of n_kv * head_dim elements, row_stride apart) to
-// position slot[t] of sequence seq[t].  One 16-byte piece per thread; bound by
-// the launch for a decode step and by memory for a prompt.
+// position slot[t] of sequence seq[t].  One 16-byte piece per thread: neighbouring
+// threads write neighbouring pieces of a row, so whole sectors move whatever the
+// strides.  Bound by the launch for a decode step (16 rows of 4 x 128: 1.7 us) and by
+// memory for a prompt (4096 such rows, 17 MB: 4.7 us, 3.6 TB/s).
 __global__ void __launch_bounds__(256) k_paged_append(PagedArgs a, const uint16_t* k, const uint16_t* v,
                                                       int64_t row_stride, const int32_t* seq, const int32_t* slot,
                                                       int T) {
@@ -42,13 +44,15 @@ __global__ void __launch_bounds__(256) k_paged_append(PagedArgs a, const uint16_
 // of all), in two launches.
 //   select   radix selection over the weights as ordered 32-bit keys, 11 + 11 + 10
 //            bits from the top: a histogram in shared memory gives the digit of the
-//            threshold key.  One CTA holds up to kEvChunk positions in registers; for
+//            threshold key.  One CTA holds up to kEvChunk positions in shared memory; for
 //            longer caches a cluster of kEvC shares them and adds its histograms up
 //            through distributed shared memory.  Ballots then give every kept position
-//            its place, in order.  (Comparing the keys with three candidates a round,
-//            two bits at a time, needs no histogram, but its sixteen rounds took 20 us
-//            where this takes 5.)
-//   move     the kept rows to places 0, 1, ... of dst.
+//            its place, in order.  Bound by the latency of its passes (12 us for 8192
+//            positions; comparing the keys with three candidates a round, two bits at a
+//            time, needs no histogram, but sixteen rounds took 20 us for 4096).
+//   move     the kept rows to places 0, 1, ... of dst: 30 us for 16 sequences of up to
+//            8192 cut to 2048 (131 MB, 4.4 TB/s).  Moved by the selecting CTAs instead,
+//            the same took 95 us: too few bytes in flight.
 constexpr int kEvC = 8, kEvThreads = 1024, kEvWarps = kEvThreads / 32;
 constexpr int kEvBins = 2048;
 constexpr int kEvRows = 8, kEvChunk = kEvRows * kEvThreads;  // positions a CTA holds at a time
@@ -315,58 +319,6 @@ __global__ void __cluster_dims__(kEvC, 1, 1) __launch_bounds__(kInPlaceThreads, 
         for (int j = m + rank * kInPlaceThreads + tid; j < e.w_stride; j += kEvC * kInPlaceThreads) wd[j] = 0.0f;
 }
 
-// ------------------------------------------------- attention, the plain kernel
-// One CTA per (query row, KV head), one warp per query head of the group: every
-// visible position in order.  weights (decode): the probabilities in a second
-// walk, the group's heads summed in order.
-template <int DT>
-__global__ void __launch_bounds__(kPagedMaxGroup * 32) k_paged_attn_rows(AttnRowsArgs p) {
-    pdl_begin();
-    using X = Elem<DT>;
-    __shared__ float s_m[kPagedMaxGroup], s_l[kPagedMaxGroup];
-    const PagedArgs& a = p.c;
-    const int t = blockIdx.x, h = blockIdx.y, g = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int s = t, i;
-    if (p.q_start) {
-        if (!find_row(a, p.q_start, t, p.T, &s, &i)) return;
-    } else {
-        i = seq_len(a, s) - 1;
-    }
-    const int nq = a.nkv * a.group, head = h * a.group + g;
-    const int hi = i + 1, lo = window_lo(i, p.window), sink_end = min(p.n_sink, lo);
-    const uint16_t* q = p.q + t * p.q_stride + head * a.hd;
-    float qf[4] = {0.0f, 0.0f, 0.0f, 0.0f}, acc[4], m, l;
-    if (4 * lane < a.hd) {
-        const uint2 w = *reinterpret_cast<const uint2*>(q + 4 * lane);
-        qf[0] = X::lo(w.x), qf[1] = X::hi(w.x), qf[2] = X::lo(w.y), qf[3] = X::hi(w.y);
-    }
-    attend_row<DT>(a, s, h, qf, p.scale, sink_end, lo, hi, acc, m, l);
-    if (4 * lane < a.hd) {
-        uint2 o = make_uint2(0, 0);  // nothing visible: zeros
-        if (hi > 0) o = make_uint2(X::pack(acc[0] / l, acc[1] / l), X::pack(acc[2] / l, acc[3] / l));
-        *reinterpret_cast<uint2*>(p.out + ((int64_t)t * nq + head) * a.hd + 4 * lane) = o;
-    }
-    if (!p.weights) return;
-    if (lane == 0) s_m[g] = m, s_l[g] = l;
-    __syncthreads();
-    float* w = p.weights + ((int64_t)s * a.nkv + h) * p.w_stride;
-    for (int j = g; j < hi; j += a.group) {
-        if (j >= sink_end && j < lo) continue;
-        const int64_t off = row_offset(a, s, j, h);
-        if (off < 0) continue;
-        float sum = 0.0f;
-        for (int gg = 0; gg < a.group; ++gg) {
-            float x = 0.0f;
-            for (int d = lane; d < a.hd; d += 32)
-                x += X::f(p.q[t * p.q_stride + (h * a.group + gg) * a.hd + d]) * X::f(a.k[off + d]);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-            sum += expf(x * p.scale - s_m[gg]) / s_l[gg];
-        }
-        if (lane == 0) w[j] += sum;
-    }
-}
-
 }  // namespace
 
 cudaError_t launch_paged_append(const PagedArgs& a, const uint16_t* k, const uint16_t* v, int64_t row_stride,
@@ -393,14 +345,6 @@ cudaError_t launch_paged_evict(const PagedArgs& src, const PagedArgs& dst, const
         r = launch_pdl(k_paged_move, dim3((most + rows - 1) / rows, src.nkv, src.n_seqs), dim3(kMoveThreads), 0, st, e);
     }
     return r != cudaSuccess ? r : cudaGetLastError();
-}
-
-cudaError_t launch_paged_attn_rows(const AttnRowsArgs& p, int dtype, cudaStream_t st) {
-    const int rows = p.q_start ? p.T : p.c.n_seqs;
-    if (rows <= 0) return cudaSuccess;
-    const cudaError_t e = launch_pdl(dtype ? k_paged_attn_rows<1> : k_paged_attn_rows<0>, dim3(rows, p.c.nkv),
-                                     dim3(32 * p.c.group), 0, st, p);
-    return e != cudaSuccess ? e : cudaGetLastError();
 }
 
 }  // namespace obs

@@ -30,6 +30,12 @@
 // rounding left: the tensor cores multiply 16-bit values, one rounding of p would
 // cost a short sequence (few p to average over) as much as the output's own, and
 // the second set of products is hidden behind the loads.
+//
+// Measured, 32 / 4 heads of 128: 32 sequences of 61 to 32768 positions in f16, pages of
+// 16: 172 us, 6.5 TB/s, 97% of the measured copy rate; 128 sequences with a window of
+// 1024 and 4 sinks 52 us (79%: each CTA starts and ends inside some item, and joining
+// takes it from loading); one of 2049 9.6 us, where the launch, four dependent accesses
+// to the first rows and the join are nearly all of it.
 #include "paged.cuh"
 
 namespace obs {
@@ -41,11 +47,6 @@ constexpr int kStages = 3;                      // per warp
 constexpr int kMinTiles = 3;                    // of a CTA's run: fewer parts to join (one sequence of 2049: 9.3 us,
                                                 // with 1 or 2 tiles 9.9 and 10.1, with 4 or 6 11.2 and 12.6)
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -73,10 +74,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// 16 bytes to shared memory, or zeros
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
 }
 
 // The visible tiles of one sequence: tiles 0 .. ts-1 (sinks), then wt .. (window).

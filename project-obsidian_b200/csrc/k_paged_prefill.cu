@@ -10,30 +10,41 @@
 // lie across the causal diagonal or the window's edge, and a chunk of a few tokens
 // still fills the tensor cores' 128 rows.
 //
-// One CTA takes one block of 256 rows, two tiles of 128 (A and B), against the
-// 128-position tiles that any of them sees (sinks, then the window):
-//   S = Q . K^T     128 x 128 fp32 in TMEM; Q and K in shared memory, K-major
+// One CTA takes one block of 256 rows, two row tiles of 128 (A and B), against the tiles
+// of 64 positions that any of its rows sees (sinks, then the window):
+//   S = Q . K^T     128 x 64 fp32 in TMEM; Q and K in shared memory, K-major
 //   P = 2^(S scale log2 e - m)   in registers, one row per thread, written back over
 //                   S as 16-bit values, the A operand of
 //   O += P . V      128 x head_dim fp32 in TMEM; V as it lies (its rows are the
 //                   reduction: the N-major form of the B operand)
+// O takes half of TMEM, the other half is two buffers of S for each row tile: S of the
+// next tile of positions is there when the softmax of one is done.  Tiles of 128
+// positions leave no second buffer, and the way from P through two products to the
+// next S is waited for (169 us instead of 157 us for one prompt of 4096).
 // Sixteen warps:
-//   0-3, 4-7   softmax of tile A, of tile B: running maximum m and sum l of the
-//              thread's row.  O is rescaled only when the maximum has grown by more
-//              than 2^8 (p stays below 2^8, far inside both types), by the same
-//              threads, between a tile's S and its P, when no product touches O
-//              The two tiles' warps of one scheduler take turns at the exponentials: in
-//              step they would share the exponential unit and then leave it idle, and
-//              both tiles' products would queue up behind one another
-//   8, 9       issue the products of tile A, of tile B: PV of a tile of positions, then
-//              QK of the tile after the next into the columns that this P leaves
+//   0-3, 4-7   softmax of row tile A, of B: running maximum m and sum l of the thread's
+//              row.  O is rescaled only when the maximum has grown by more than 2^8 (p
+//              stays below 2^8, far inside both types), by the same threads, between a
+//              tile's S and its P, when no product touches O.  The two row tiles' warps
+//              of one scheduler take turns at the exponentials: in step they would share
+//              the exponential unit and then leave it idle, and both row tiles' products
+//              would queue up behind one another (157 -> 145 us)
+//   8, 9       issue the products of A, of B: PV of a tile of positions, then QK of the
+//              tile after the next into the columns that this P leaves
 //   12-15      loads: rows of K and V by page, 16 bytes per cp.async, into the
 //              128-byte-swizzled tiles (rows that no query of the block sees as zeros);
 //              a stage's barrier counts the pieces as they land, and the fence that lets
 //              the tensor cores see them is the issuing warp's (in the loading warps it
 //              would wait for every load in flight)
-// What bounds it: for head_dim 128 the exponentials (16 a clock and SM) take as long
-// as the products (8192 operations a clock).
+// Measured for 32 / 4 heads of 128 in bf16: one prompt of 4096 137 us, 1.0 PFLOP/s, 60% of
+// the measured bf16 rate (up to 154 us, 53%, with the clock under its power limit); one
+// of 8192 with a window of 1024 and 4 sinks 177 us, 730 TFLOP/s.  What bounds it: a tile
+// takes 1770 cycles a block, of which the exponentials (64 a row at 16 a clock and SM)
+// need 1024 and the products 1370 (390 for a 128 x 64 x 128 QK, whose operands come from
+// shared memory at its full rate, 294 for a PV); half the products left out saves 5%,
+// no loads at all nothing, so the rest is the softmax warps' own latency from S to P.
+// A block's start (finding it, Q, the first tiles) and end cost 9000 cycles, a fifth of
+// a window of 1024.
 //
 // p is rounded to 16 bits once; over many positions the roundings average out far
 // below the output's own.  Where a row of the block sees fewer than kFewKeys
@@ -91,11 +102,6 @@ __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile
         }
     }
 }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -122,9 +128,6 @@ __device__ __forceinline__ void add2(float& s0, float& s1, float a0, float a1) {
         "mov.b64 {%0, %1}, s;\n\t}"
         : "+f"(s0), "+f"(s1)
         : "f"(a0), "f"(a1));
-}
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
 }
 // 32 lanes x 32 consecutive fp32 columns (no wait)
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {

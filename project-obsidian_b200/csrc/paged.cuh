@@ -86,18 +86,6 @@ __device__ __forceinline__ bool find_row(const PagedArgs& a, const int32_t* q_st
     return true;
 }
 
-struct AttnRowsArgs {
-    PagedArgs c;
-    const uint16_t* q;        // [rows][nq][hd], rows q_stride elements apart
-    int64_t q_stride;
-    uint16_t* out;            // [rows][nq][hd]
-    const int32_t* q_start;   // prefill: [n_seqs + 1]; decode: null, row t is sequence t's last position
-    int T;                    // prefill: rows
-    int window, n_sink;
-    float scale;
-    float* weights;           // decode, optional: [n_seqs][nkv][w_stride]
-    int w_stride;
-};
 constexpr int kPagedCtas = 2;  // CTAs per SM of the decode kernel
 struct DecodeArgs {
     PagedArgs c;
@@ -139,7 +127,6 @@ cudaError_t launch_paged_append(const PagedArgs& a, const uint16_t* k, const uin
                                 const int32_t* seq, const int32_t* slot, int T, int num_sms, cudaStream_t st);
 cudaError_t launch_paged_evict(const PagedArgs& src, const PagedArgs& dst, const float* w, float* w_dst, int w_stride,
                                int budget, int n_sink, int n_recent, int32_t* kept, int32_t* new_len, cudaStream_t st);
-cudaError_t launch_paged_attn_rows(const AttnRowsArgs& p, int dtype, cudaStream_t st);
 
 // 16-bit element types: bf16 (0) and f16 (1)
 template <int DT>
@@ -163,6 +150,16 @@ struct Elem<1> {
         return *reinterpret_cast<const uint32_t*>(&v);
     }
 };
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 16 bytes to shared memory without passing the registers, or zeros
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
 
 // One query row against its visible positions, one warp, scalar (lane l holds the
 // four dimensions 4l .. 4l+3): the online softmax in the order of the positions.

@@ -2,10 +2,13 @@
 the bounds the kernels' outputs are held to.
 
 Bound of an attention output o = sum_j p_j v_j against the exact value, element by
-element, with u the rounding of the 16-bit type (2^-9 bf16, 2^-12 f16) and
-A = sum_j p_j |v_j|:
-    u |o|          the one rounding of the output
-  + u A            each p_j is rounded to the type for the product with v
+element, with u half the unit roundoff of the 16-bit type (u = 2^-9 bf16, 2^-12 f16)
+and A = sum_j p_j |v_j| >= |o|:
+    u |o| + u A    the one rounding of the output takes 2 u |o| at most; what is left,
+                   u (A - |o|), is for p where it is rounded to the type for the product
+                   with v, which is therefore allowed only where many p average out (the
+                   decode carries p in two pieces, the prefill does for rows that see few
+                   positions)
   + 1e-4 A         fp32 scores and exponentials: a score is a sum of head_dim <= 128
                    products, off by at most 128 * 2^-24 * sum |q k| * scale; for rows of
                    unit normal entries sum |q k| scale <= 128 / sqrt(128) = 11.3 on average,
