@@ -50,8 +50,8 @@ __global__ void __launch_bounds__(256) k_paged_append(PagedArgs a, const uint16_
 //            its place, in order.  Bound by the latency of its passes (12 us for 8192
 //            positions; comparing the keys with three candidates a round, two bits at a
 //            time, needs no histogram, but sixteen rounds took 20 us for 4096).
-//   move     the kept rows to places 0, 1, ... of dst: 30 us for 16 sequences of up to
-//            8192 cut to 2048 (131 MB, 4.4 TB/s).  Moved by the selecting CTAs instead,
+//   move     the kept rows to places 0, 1, ... of dst by CTAs of a few rows: with the
+//            selection 42 us for 16 sequences of up to 8192 cut to 2048 (131 MB).  Moved by the selecting CTAs instead,
 //            the same took 95 us: too few bytes in flight.
 constexpr int kEvC = 8, kEvThreads = 1024, kEvWarps = kEvThreads / 32;
 constexpr int kEvBins = 2048;
@@ -237,7 +237,8 @@ __global__ void __launch_bounds__(kEvThreads) k_paged_select(EvictArgs e) {
 // ---- move, to pages that the source does not hold: one warp (or two half ones) per
 // kept row, a 16-byte piece of K or V per lane, kMoveU rows each; enough in flight
 // for the memory's rate.  The weights move along, the rest of their row is cleared.
-constexpr int kMoveU = 4, kMoveThreads = 256, kInPlaceThreads = 512;
+constexpr int kMoveU = 2, kMoveThreads = 128;          // (4 rows by 256 threads: 51 us instead of 42 us for the whole eviction)
+constexpr int kInPlaceU = 4, kInPlaceThreads = 512;
 
 __global__ void __launch_bounds__(kMoveThreads) k_paged_move(EvictArgs e) {
     pdl_begin();
@@ -290,13 +291,13 @@ __global__ void __cluster_dims__(kEvC, 1, 1) __launch_bounds__(kInPlaceThreads, 
     const int lr = tid / per_row, c = tid - lr * per_row, piece = (c >= pieces ? c - pieces : c) * 8;
     const uint16_t* from = c >= pieces ? a.v : a.k;
     uint16_t* to = const_cast<uint16_t*>(c >= pieces ? e.dst.v : e.dst.k);
-    const int step = kEvC * rows_cta * kMoveU;
+    const int step = kEvC * rows_cta * kInPlaceU;
     for (int c0 = 0; c0 < m; c0 += step) {
-        int64_t dst[kMoveU];
-        uint4 x[kMoveU];
-        float wv[kMoveU];
+        int64_t dst[kInPlaceU];
+        uint4 x[kInPlaceU];
+        float wv[kInPlaceU];
 #pragma unroll
-        for (int u = 0; u < kMoveU; ++u) {
+        for (int u = 0; u < kInPlaceU; ++u) {
             const int j = c0 + (u * kEvC + rank) * rows_cta + lr;
             dst[u] = -1, wv[u] = 0.0f;
             if (lr < rows_cta && j < m) {
@@ -308,7 +309,7 @@ __global__ void __cluster_dims__(kEvC, 1, 1) __launch_bounds__(kInPlaceThreads, 
         }
         cl.sync();
 #pragma unroll
-        for (int u = 0; u < kMoveU; ++u) {
+        for (int u = 0; u < kInPlaceU; ++u) {
             const int j = c0 + (u * kEvC + rank) * rows_cta + lr;
             if (dst[u] >= 0) *reinterpret_cast<uint4*>(to + dst[u] + piece) = x[u];
             if (wd && lr < rows_cta && j < m && c == 0) wd[j] = wv[u];
