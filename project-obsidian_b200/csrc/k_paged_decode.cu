@@ -31,6 +31,10 @@
 // cost a short sequence (few p to average over) as much as the output's own, and
 // the second set of products is hidden behind the loads.
 //
+// An infinity in V times what rounding left of its p, zero or negative, would be NaN: a
+// head whose sums are not finite although its l is takes its positions again one by one
+// (attend_row).  When nothing is wrong this costs a comparison.
+//
 // Measured, 32 / 4 heads of 128: 32 sequences of 61 to 32768 positions in f16, pages of
 // 16: 172 us, 6.5 TB/s, 97% of the measured copy rate; 128 sequences with a window of
 // 1024 and 4 sinks 52 us (79%: each CTA starts and ends inside some item, and joining
@@ -111,6 +115,28 @@ __device__ __forceinline__ void advance(const PagedArgs& a, int window, int n_si
 
 // one part: group rows of HD sums, then group (maximum, sum) pairs; 16-byte aligned
 __host__ __device__ constexpr int part_floats(int group, int hd) { return group * hd + (2 * group + 3) / 4 * 4; }
+
+__device__ __forceinline__ bool needs_again(const float (&o)[4], float l) {
+    const float z = o[0] * 0.0f + o[1] * 0.0f + (o[2] * 0.0f + o[3] * 0.0f);  // NaN unless all are finite
+    return z != 0.0f && l > 0.0f && l <= 3.4e38f;
+}
+// One head once more, by a warp.
+template <int DT>
+__device__ __forceinline__ void again(const DecodeArgs& p, int s, int h, int head, int sink_end, int lo, int n) {
+    using X = Elem<DT>;
+    const PagedArgs& a = p.c;
+    const int lane = threadIdx.x & 31;
+    const int64_t at = (h * a.group + head) * a.hd + 4 * lane;
+    float qf[4] = {0.0f, 0.0f, 0.0f, 0.0f}, acc[4], m, l;
+    if (4 * lane < a.hd) {
+        const uint2 w = *reinterpret_cast<const uint2*>(p.q + s * p.q_stride + at);
+        qf[0] = X::lo(w.x), qf[1] = X::hi(w.x), qf[2] = X::lo(w.y), qf[3] = X::hi(w.y);
+    }
+    attend_row<DT>(a, s, h, qf, p.scale, sink_end, lo, n, acc, m, l);
+    if (4 * lane < a.hd)
+        *reinterpret_cast<uint2*>(p.out + (int64_t)s * a.nkv * a.group * a.hd + at) =
+            make_uint2(X::pack(acc[0] / l, acc[1] / l), X::pack(acc[2] / l, acc[3] / l));
+}
 
 template <int HD>
 struct DecodeSmem {
@@ -383,6 +409,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
             }
         __syncthreads();
         const int hsub = tid >> 4, dsub = (tid & 15) * 4;  // of 8 heads x 64 dimensions
+        uint32_t bad = 0;  // heads this thread has written a sum of that is not finite, with l > 0 that is
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int head = nt * 8 + hsub;
@@ -415,6 +442,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
                             uint16_t* dst = p.out + ((int64_t)cs.s * nq + cs.h * G + head) * a.hd + d;
                             *reinterpret_cast<uint2*>(dst) =
                                 make_uint2(X::pack(o[0] / ls, o[1] / ls), X::pack(o[2] / ls, o[3] / ls));
+                            bad |= (uint32_t)needs_again(o, ls) << head;
                         }
                     } else {
                         *reinterpret_cast<float4*>(part + head * HD + d) = make_float4(o[0], o[1], o[2], o[3]);
@@ -494,11 +522,18 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
                         uint16_t* dst = p.out + ((int64_t)cs.s * nq + cs.h * G + head) * a.hd + d;
                         *reinterpret_cast<uint2*>(dst) = make_uint2(X::pack(o[r][0] / L[r], o[r][1] / L[r]),
                                                                     X::pack(o[r][2] / L[r], o[r][3] / L[r]));
+                        bad |= (uint32_t)needs_again(o[r], L[r]) << head;
                         if (p.ml && d == 0)
                             p.ml[(int64_t)cs.s * nq + cs.h * G + head] = make_float2(M[r] == -INFINITY ? 0.0f : M[r], L[r]);
                     }
                 }
             }
+        }
+        bad = __reduce_or_sync(0xffffffffu, bad);  // (a warp writes all of a head)
+        while (bad) {
+            const int head = __ffs(bad) - 1;
+            bad &= bad - 1;
+            again<DT>(p, cs.s, cs.h, head, cs.sp.sink_end, cs.sp.lo, cs.sp.n);
         }
         __syncthreads();  // s_m, s_l and s_mrg are written again by the next run
         fresh = true;

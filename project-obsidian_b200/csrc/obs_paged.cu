@@ -171,7 +171,7 @@ extern "C" int obs_paged_decode(obs_ctx* ctx, const obs_paged_kv* kv, const void
     if (weights && w_stride < a.cap) a.cap = w_stride;  // a longer sequence is refused on the device
     const float sc = scale > 0.0f ? scale : 1.0f / sqrtf((float)a.hd);
     DecodeArgs p{a, reinterpret_cast<const uint16_t*>(q), q_stride, reinterpret_cast<uint16_t*>(out), window, n_sink,
-                 sc * kLog2e, ps->part, ps->count, weights ? ps->scores : nullptr, ps->cfg.max_kv_len,
+                 sc, sc * kLog2e, ps->part, ps->count, weights ? ps->scores : nullptr, ps->cfg.max_kv_len,
                  (a.group + 1) & ~1,
                  weights ? ps->ml : nullptr, weights, w_stride};
     return launched(ctx, launch_paged_decode(p, ps->cfg.dtype, parts.num_sms, as_stream(stream)), "paged decode");

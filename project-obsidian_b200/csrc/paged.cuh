@@ -93,7 +93,7 @@ struct DecodeArgs {
     int64_t q_stride;
     uint16_t* out;            // [n_seqs][nq][hd]
     int window, n_sink;
-    float scale_log2;         // scale * log2(e)
+    float scale, scale_log2;  // scale_log2 = scale * log2(e)
     float* part;              // 2 per CTA: its parts of (sequence, head)s it shares
     uint32_t* count;          // [CTAs] arrivals, zero between launches
     float* scores;            // with weights: [n_seqs][nkv][score_ld][score_heads] x_j

@@ -579,3 +579,48 @@ def test_host_refusals(torch_):
     ctx.paged_decode(kv, q, out)
     ctx.check_device()
     ctx.close()
+
+
+# ------------------------------------------------- values at the types' ends
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("heads,kv,hd,ln", [(8, 1, 128, 20), (8, 1, 128, 9000), (6, 2, 64, 700), (32, 2, 120, 300)])
+def test_infinite_values_stay_in_their_dimension(torch_, dtype, heads, kv, hd, ln):
+    """p v_j of a visible infinity is that infinity, of a NaN NaN, for the queries that see it and in its dimension
+    alone; both infinities in one dimension give NaN."""
+    from paged_util import Cache, attend, check_out, visible
+
+    torch = torch_
+    group, inf = heads // kv, float("inf")
+    c = Cache([ln, 40], kv, hd, 16, dtype, seed=90)
+    ctx = make_ctx(heads, kv, hd, 16, dtype, max_len=9000)
+    rows = 3
+    q = queries(torch, 2 * rows, heads, hd, c.dtype, 90)
+    start = torch.tensor([0, rows, 2 * rows], dtype=torch.int32, device="cuda")
+    bad = {(5, 0): inf, (6, 3): -inf, (7, 4): float("nan"), (8, 7): inf, (9, 7): -inf}
+    want = {0: inf, 3: -inf, 4: float("nan"), 7: float("nan")}
+    for (j, d), x in bad.items():
+        p, o = c.places(0, torch.tensor([j], device="cuda"))
+        c.v[p, o, kv - 1, d] = x
+    out = torch.zeros((2 * rows, heads, hd), dtype=c.dtype, device="cuda")
+    ctx.paged_prefill(view(c), q, out, start, 2 * rows)
+    last = torch.zeros((2, heads, hd), dtype=c.dtype, device="cuda")
+    ctx.paged_decode(view(c), q[rows - 1::rows].contiguous(), last)
+    ctx.check_device()
+    for got, at in ((out, (0, rows)), (last, (0, 1))):
+        n = rows if got is out else 1
+        for s, length in enumerate(c.lens):
+            ok = visible(torch.arange(length - n, length, device="cuda"), length, 0, 0)
+            k, v = c.rows(s, length)
+            for h in range(kv):
+                sees = s == 0 and h == kv - 1
+                mine = got[at[s]:at[s] + n, h * group:(h + 1) * group].clone()
+                qs = q[rows * s + rows - n:rows * (s + 1), h * group:(h + 1) * group]
+                vv = v[:, h].clone()
+                if sees:
+                    for d, x in want.items():
+                        assert torch.equal(mine[..., d].float().nan_to_num(nan=7.0, posinf=8.0, neginf=9.0),
+                                           torch.full_like(mine[..., d], 7.0 if x != x else 8.0 if x > 0 else 9.0).float()), d
+                        mine[..., d], vv[:, d] = 0.0, 0.0
+                o, a, sv, _ = attend(qs, k[:, h], vv, ok, hd ** -0.5)
+                check_out(mine, o, a, sv, c.dtype)
+    ctx.close()
