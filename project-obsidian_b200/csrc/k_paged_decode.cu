@@ -31,6 +31,9 @@
 // cost a short sequence (few p to average over) as much as the output's own, and
 // the second set of products is hidden behind the loads.
 //
+// f16 holds nothing below 2^-25, and a first position that many scores fall 2^25 behind
+// is common: p <= 1 is multiplied by 2^15 there, and the sums by 2^-15 at their end.
+//
 // An infinity in V times what rounding left of its p, zero or negative, would be NaN: a
 // head whose sums are not finite although its l is takes its positions again one by one
 // (attend_row).  When nothing is wrong this costs a comparison.
@@ -153,6 +156,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
     pdl_begin();
     using X = Elem<DT>;
     using M = DecodeSmem<HD>;
+    constexpr float kScaleP = DT == 0 ? 1.0f : 32768.0f;
     extern __shared__ __align__(1024) uint8_t smem[];
     float* s_mrg = reinterpret_cast<float*>(smem + M::RING);
     __shared__ float s_m[kWarps][16], s_l[kWarps][16];
@@ -369,9 +373,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
             }
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const uint32_t hi = X::pack(x[2 * r], x[2 * r + 1]);
+                const float x0 = x[2 * r] * kScaleP, x1 = x[2 * r + 1] * kScaleP;
+                const uint32_t hi = X::pack(x0, x1);
                 pb[nt][r] = movm(hi);
-                pr[nt][r] = movm(X::pack(x[2 * r] - X::lo(hi), x[2 * r + 1] - X::hi(hi)));
+                pr[nt][r] = movm(X::pack(x0 - X::lo(hi), x1 - X::hi(hi)));
             }
         }
 #pragma unroll
@@ -418,7 +423,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
             for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, s_m[w][head]);
             const float ref = mx == -INFINITY ? 0.0f : mx;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) mw[w] = ex2(s_m[w][head] - ref), ls += mw[w] * s_l[w][head];
+            for (int w = 0; w < kWarps; ++w) {
+                mw[w] = ex2(s_m[w][head] - ref), ls += mw[w] * s_l[w][head];
+                mw[w] *= 1.0f / kScaleP;  // of the sums of p v
+            }
 #pragma unroll
             for (int half = 0; half < HD / 64; ++half) {
                 if (nt || half) __syncthreads();

@@ -52,6 +52,10 @@
 // half of S's columns holds it): half as much work again for the first tiles of a
 // prompt.
 //
+// f16 holds nothing below 2^-25, and a first position that many scores fall 2^25 behind
+// is common: there p is 2^7 times as large (2^15 at most, with what the maximum may have
+// grown by), and so are l and O.
+//
 // A NaN or infinity in V meets p = 0 of rows that do not see it, and 0 * NaN is NaN:
 // a row whose result is not finite is computed again from its visible positions
 // alone (attend_row).  When nothing is wrong this costs a comparison.
@@ -220,6 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
     pdl_begin();
     using X = Elem<DT>;
     using C = Pf<HD>;
+    constexpr float kShift = DT == 0 ? 0.0f : 7.0f;  // p is taken against m - kShift
     extern __shared__ uint8_t smem_raw[];
     __shared__ int s_scan[kThreads / 32];
     __shared__ int s_blk[5];  // sequence, block of it, its rows' range, its length
@@ -574,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
                 ok = false;
                 break;
             }
-            const float ref = m == -INFINITY ? 0.0f : m;
+            const float ref = m == -INFINITY ? 0.0f : m - kShift;
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int c0 = 0; c0 < kKeys; c0 += 32) {
@@ -610,7 +615,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
             const int64_t row = (int64_t)t * nq + head;
             float2 fin = make_float2(0.0f, 0.0f);
             uint8_t* stg = smem + x * C::QTILE + (warp & 3) * 4096;
-            if (split && valid) p.part_ml[(int64_t)z * p.T * nq + row] = make_float2(m, l);
+            if (split && valid) p.part_ml[(int64_t)z * p.T * nq + row] = make_float2(m - kShift, l);
             const float inv = i < 0 ? 1.0f : 1.0f / l;
 #pragma unroll
             for (int c = 0; c < HD; c += 64) {

@@ -624,3 +624,34 @@ def test_infinite_values_stay_in_their_dimension(torch_, dtype, heads, kv, hd, l
                 o, a, sv, _ = attend(qs, k[:, h], vv, ok, hd ** -0.5)
                 check_out(mine, o, a, sv, c.dtype)
     ctx.close()
+
+
+def test_f16_many_small_probabilities(torch_):
+    """A first position whose score lies 26 powers of two above 65535 equal ones, in heads enough that no CTA sees
+    few of them: what the small ones add up to is there.  The bound of paged_util with its term for p below the
+    smallest normal f16, 2^-24 S, as it is for p multiplied by 2^15 (decode) and 2^7 (prefill)."""
+    from paged_util import Cache, attend, visible, U
+
+    torch = torch_
+    ln, kv, hd = 65536, 160, 8
+    c = Cache([ln], kv, hd, 64, "f16", seed=91)
+    j = torch.arange(ln, device="cuda")
+    k, v = torch.zeros_like(c.kd[0]), c.vd[0].abs()
+    k[0], v[0] = 18.0 / hd, 0.0
+    c.put(0, j, k, v)
+    ctx = make_ctx(kv, kv, hd, 64, "f16", max_len=ln)
+    q = torch.ones((1, kv, hd), dtype=c.dtype, device="cuda")
+    start = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    one, two = torch.zeros_like(q), torch.zeros_like(q)
+    ctx.paged_decode(view(c), q, one, scale=1.0)
+    ctx.paged_prefill(view(c), q, two, start, 1, scale=1.0)
+    ctx.check_device()
+    ok, u = visible(j[-1:], ln, 0, 0), U[c.dtype]
+    for h in range(kv):
+        o, a, sv, _ = attend(q[:, h:h + 1], k[:, h], v[:, h], ok, 1.0)
+        for got, shift in ((one, 15), (two, 7)):
+            # (the output itself may lie below the smallest normal f16: 2^-25)
+            bound = u * o.abs() + (u + 1e-4) * a + 2.0 ** (-24 - shift) * sv + 2.0 ** -25
+            worst = float(((got[:, h:h + 1].double() - o).abs() / bound).max())
+            assert worst <= 1.0, f"head {h}, shift {shift}: {worst:.3f} times the bound"
+    ctx.close()
