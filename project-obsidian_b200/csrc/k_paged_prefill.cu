@@ -58,7 +58,9 @@
 //
 // A NaN or infinity in V meets p = 0 of rows that do not see it, and 0 * NaN is NaN:
 // a row whose result is not finite is computed again from its visible positions
-// alone (attend_row).  When nothing is wrong this costs a comparison.
+// alone (attend_row), unless l says that its own scores are the reason (NaN or +inf
+// among them, or all -inf: the whole row is NaN).  When nothing is wrong this costs a
+// comparison.
 //
 // Few rows, long axis: where there are fewer blocks than SMs the tiles of a block
 // are split over several CTAs, whose (m, l, O) k_paged_join puts together in order.
@@ -658,7 +660,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
                     }
                 }
             }
-            uint32_t again = __ballot_sync(0xffffffffu, valid && i >= 0 && !(fin.x + fin.y == 0.0f) && !split);
+            uint32_t again = __ballot_sync(0xffffffffu, valid && i >= 0 && !(fin.x + fin.y == 0.0f) && l > 0.0f && l <= 3.4e38f && !split);
             while (again) {  // (never with split: k_paged_join does it)
                 const int who = __ffs(again) - 1;
                 again &= again - 1;
@@ -730,7 +732,7 @@ __global__ void __launch_bounds__(256) k_paged_join(PrefillArgs p) {
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
         o[e] = i < 0 ? 0.0f : o[e] / l;
-        bad |= !(fabsf(o[e]) <= 3.4e38f);
+        bad |= !(fabsf(o[e]) <= 3.4e38f) && l > 0.0f && l <= 3.4e38f;
     }
     const int d = lane * PER;
     if (d < a.hd) {
