@@ -237,8 +237,9 @@ int obs_kv_read(obs_ctx* ctx, int layer, int seq, int pos0, int n, uint16_t* k, 
  * lengths; a call is given one layer's cache (obs_paged_kv).  Tables and lengths
  * are read on the device, in stream order, so a captured CUDA graph serves
  * growing sequences.  A page id outside the pool or a length beyond the table
- * (or max_kv_len, or a weights row) is refused on the device: such rows are left
- * out and obs_check_device reports OBS_ERR_INVALID.
+ * (or max_kv_len, or a weights row) is refused on the device: nothing outside is
+ * read or written (such rows count as zeros, such a length as the largest) and
+ * obs_check_device reports OBS_ERR_INVALID.
  *
  * obs_paged_init: the shape that the calls below take and their workspace, once
  * per context (independent of obs_attn_init and of the number of layers). */

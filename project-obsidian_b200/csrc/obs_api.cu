@@ -690,6 +690,8 @@ extern "C" int obs_paged_attn_forward(obs_ctx* ctx, int layer, const obs_paged_k
     if (out == x) return fail(ctx, OBS_ERR_INVALID, "out may not alias x");
     if (!q_start && T != kv->n_seqs) return fail(ctx, OBS_ERR_INVALID, "a decode step (q_start NULL) has one token per sequence");
     if (q_start && weights) return fail(ctx, OBS_ERR_UNSUPPORTED, "weights are added up by decode steps only");
+    int rc = paged_check(ctx, kv, !q_start, window, n_sink, weights, w_stride);  // (a refused call appends nothing)
+    if (rc != OBS_OK) return rc;
     cudaStream_t st = as_stream(stream);
     uint16_t* krows = ctx->a_kv;
     uint16_t* vrows = ctx->a_kv + (size_t)ctx->cfg.max_tokens * nkv * hd;
@@ -699,7 +701,7 @@ extern "C" int obs_paged_attn_forward(obs_ctx* ctx, int layer, const obs_paged_k
     CU(launch_qk_norm_rope(ctx->a_qkv, T, nq, nkv, hd, L.q_norm, L.k_norm, ctx->cfg.rms_eps, ctx->rope_cs, ac.max_seq,
                            seq, pos, ctx->a_q, krows, vrows, kv->n_seqs, ctx->err_flag, st, 1),
        "q/k norm, rope");
-    int rc = obs_paged_append(ctx, kv, krows, vrows, (int64_t)nkv * hd, seq, slot, T, stream);
+    rc = obs_paged_append(ctx, kv, krows, vrows, (int64_t)nkv * hd, seq, slot, T, stream);
     if (rc == OBS_OK)
         rc = q_start ? obs_paged_prefill(ctx, kv, ctx->a_q, (int64_t)nq * hd, ctx->a_out, q_start, T, window, n_sink, 0.0f,
                                          stream)

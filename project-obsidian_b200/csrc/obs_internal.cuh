@@ -266,6 +266,12 @@ struct CtxParts {
 CtxParts ctx_parts(obs_ctx* ctx);
 // the caller's cache must be the attention block's: heads, KV heads, head_dim, bf16 (else a message)
 const char* paged_mismatch(const PagedState* p, int nq, int nkv, int hd);
+}  // namespace obs
+struct obs_paged_kv;
+namespace obs {
+// what append and decode or prefill would refuse, before the first of them is launched
+int paged_check(obs_ctx* ctx, const obs_paged_kv* kv, bool decode, int window, int n_sink, const float* weights,
+                int w_stride);
 
 // ----------------------------------------------------------------- k_gemm.cu
 enum GemmEpi : int { kEpiSwiglu = 0, kEpiBf16 = 1, kEpiF32 = 2 };

@@ -80,6 +80,18 @@ const char* query_args(const PagedArgs& a, const void* q, int64_t q_stride, cons
     return nullptr;
 }
 
+const char* decode_args(const PagedState* ps, const PagedArgs& a, const float* weights, int w_stride, int* code) {
+    *code = OBS_ERR_INVALID;
+    if ((int64_t)a.n_seqs * a.nkv * (a.cap / 64 + 2) > 0x7fffffff)
+        return "n_seqs * n_kv_heads * positions is too large for one call";
+    if (weights && !ps->cfg.weights) {
+        *code = OBS_ERR_STATE;
+        return "the paged cache was initialised without room for weights";
+    }
+    if (weights && w_stride <= 0) return "w_stride must be positive";
+    return nullptr;
+}
+
 #define PAGED_BEGIN()                                                                                             \
     if (!ctx) return OBS_ERR_INVALID;                                                                             \
     const CtxParts parts = ctx_parts(ctx);                                                                        \
@@ -98,6 +110,17 @@ int launched(obs_ctx* ctx, cudaError_t e, const char* what) {
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
 }  // namespace
+
+int obs::paged_check(obs_ctx* ctx, const obs_paged_kv* kv, bool decode, int window, int n_sink, const float* weights,
+                     int w_stride) {
+    PAGED_BEGIN();
+    if (window < 0 || n_sink < 0) return ctx_fail(ctx, OBS_ERR_INVALID, "window and n_sink must not be negative");
+    if (a.n_seqs == 0) return ctx_fail(ctx, OBS_ERR_INVALID, "rows without sequences");
+    int code;
+    if (decode)
+        if (const char* m = decode_args(ps, a, weights, w_stride, &code)) return ctx_fail(ctx, code, m);
+    return OBS_OK;
+}
 
 extern "C" int obs_paged_init(obs_ctx* ctx, const obs_paged_config* cfg) {
     if (!ctx) return OBS_ERR_INVALID;
@@ -163,11 +186,8 @@ extern "C" int obs_paged_decode(obs_ctx* ctx, const obs_paged_kv* kv, const void
     PAGED_BEGIN();
     if (a.n_seqs == 0) return OBS_OK;
     if (const char* m = query_args(a, q, q_stride, out, window, n_sink, scale)) return ctx_fail(ctx, OBS_ERR_INVALID, m);
-    if ((int64_t)a.n_seqs * a.nkv * (a.cap / 64 + 2) > 0x7fffffff)
-        return ctx_fail(ctx, OBS_ERR_INVALID, "n_seqs * n_kv_heads * positions is too large for one call");
-    if (weights && !ps->cfg.weights)
-        return ctx_fail(ctx, OBS_ERR_STATE, "the paged cache was initialised without room for weights");
-    if (weights && w_stride <= 0) return ctx_fail(ctx, OBS_ERR_INVALID, "w_stride must be positive");
+    int code;
+    if (const char* m = decode_args(ps, a, weights, w_stride, &code)) return ctx_fail(ctx, code, m);
     if (weights && w_stride < a.cap) a.cap = w_stride;  // a longer sequence is refused on the device
     const float sc = scale > 0.0f ? scale : 1.0f / sqrtf((float)a.hd);
     DecodeArgs p{a, reinterpret_cast<const uint16_t*>(q), q_stride, reinterpret_cast<uint16_t*>(out), window, n_sink,

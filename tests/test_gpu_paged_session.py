@@ -95,6 +95,31 @@ def test_paged_block_refusals(pair):
     other.close()
 
 
+@pytest.mark.parametrize("kw,msg", [(dict(window=-1), "negative"), (dict(n_sink=-1), "negative"),
+                                    (dict(weights=True), "without room for weights")])
+def test_a_refused_step_appends_nothing(cuda, kw, msg):
+    torch = cuda
+    ctx = obsmoe.MoeContext(obsmoe.MoeShape(H, 256, 16, 4, n_layers=1, max_tokens=4), 0)
+    ctx.attn_init(NQ, NKV, HD, 32, 1, THETA)
+    ctx.load_attn(0, O.synth_attn(seed=9, layer=0, H=H, nq=NQ, nkv=NKV, hd=HD))
+    ctx.paged_init(NQ, NKV, HD, PAGE, max_seqs=1, max_kv_len=32)
+    k, v = (torch.zeros((2, PAGE, NKV, HD), dtype=torch.bfloat16, device="cuda") for _ in "kv")
+    zero, one = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+    kv = obsmoe.PagedKV(k, v, torch.tensor([[0, 1]], dtype=torch.int32, device="cuda"), one)
+    x = dev(torch, O.synth_x(5, 0, 1, H))
+    y = torch.empty_like(x)
+    if "weights" in kw:
+        kw = dict(weights=torch.zeros((1, NKV, 32), device="cuda"))
+    with pytest.raises(obsmoe.ObsError, match=msg):
+        ctx.paged_attn_forward(0, kv, x, y, 1, zero, zero, zero, **kw)
+    torch.cuda.synchronize()
+    assert not k.any() and not v.any()
+    ctx.paged_attn_forward(0, kv, x, y, 1, zero, zero, zero)
+    ctx.check_device()
+    assert k[0, 0].any() and v[0, 0].any()
+    ctx.close()
+
+
 @pytest.fixture(scope="module")
 def example(cuda):
     sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples"))
