@@ -538,6 +538,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
             }
         }
         bad = __reduce_or_sync(0xffffffffu, bad);  // (a warp writes all of a head)
+        __syncwarp();  // the head's first values before the second, which other lanes store
         while (bad) {
             const int head = __ffs(bad) - 1;
             bad &= bad - 1;

@@ -661,6 +661,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
                 }
             }
             uint32_t again = __ballot_sync(0xffffffffu, valid && i >= 0 && !(fin.x + fin.y == 0.0f) && l > 0.0f && l <= 3.4e38f && !split);
+            __syncwarp();  // the rows' first values before the second, which other lanes store
             while (again) {  // (never with split: k_paged_join does it)
                 const int who = __ffs(again) - 1;
                 again &= again - 1;
