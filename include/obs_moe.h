@@ -287,7 +287,11 @@ int obs_paged_evict(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_kv* ds
  * token t is sequence t's; weights optional) or obs_paged_prefill (q_start as
  * there), the o projection and the residual.  kv->kv_len already counts this call's
  * tokens.  Needs obs_attn_init, obs_load_attn and obs_paged_init of the same heads
- * and head_dim in bf16; the dense caches are not used. */
+ * and head_dim in bf16; the dense caches are not used.  pos[t] is below
+ * obs_attn_config.max_seq (<= 40960), the RoPE table's end, however long the cache may
+ * be and however much of it has been evicted: a token beyond it, or one with a sequence
+ * or slot outside the cache, is refused on the device (OBS_ERR_INVALID from
+ * obs_check_device); nothing is appended for it. */
 int obs_paged_attn_forward(obs_ctx* ctx, int layer, const obs_paged_kv* kv, const uint16_t* x, uint16_t* out, int T,
                            const int32_t* seq, const int32_t* pos, const int32_t* slot, const int32_t* q_start,
                            int window, int n_sink, float* weights, int w_stride, void* stream);

@@ -42,7 +42,8 @@ __device__ __forceinline__ void rope_pair(float x0, float x1, float c, float s, 
 // (256 "threads" strided over hd, halving tree) -- here 128 threads carry the
 // first 128 partials and the upper 128 are zero, which is the same sum.  kv_rows:
 // K and V go to row t of kcache / vcache ([T][nkv][hd], for a paged cache's append)
-// instead of the sequence's cache.
+// instead of the sequence's cache; a refused token's rows of q, K and V are zeros there,
+// not what an earlier call left.
 __global__ void __launch_bounds__(kAttnThreads) k_qk_norm_rope(const float* qkv, int T, int nq, int nkv,
                                                                int hd, const uint16_t* __restrict__ qn,
                                                                const uint16_t* __restrict__ kn, float eps,
@@ -62,6 +63,10 @@ __global__ void __launch_bounds__(kAttnThreads) k_qk_norm_rope(const float* qkv,
     const int s_id = seq[t], p = pos[t];
     if (s_id < 0 || s_id >= n_seqs || p < 0 || p >= max_seq) {
         if (l == 0) atomicExch(err, kDevBadPos);
+        if (kv_rows && l < hd) {
+            if (isq) qout[((size_t)t * nq + h) * hd + l] = 0;
+            else kcache[((size_t)t * nkv + hh) * hd + l] = vcache[((size_t)t * nkv + hh) * hd + l] = 0;
+        }
         return;
     }
     // the projection rounded to bf16 (the reference's half output), then the head norm

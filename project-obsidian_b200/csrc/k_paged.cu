@@ -11,13 +11,14 @@ namespace obs {
 namespace {
 
 // Row t of k and v ([T] rows of n_kv * head_dim elements, row_stride apart) to
-// position slot[t] of sequence seq[t].  One 16-byte piece per thread: neighbouring
+// position slot[t] of sequence seq[t]; with `pos`, a row whose pos[t] lies outside
+// [0, max_pos) is refused like one outside the cache.  One 16-byte piece per thread: neighbouring
 // threads write neighbouring pieces of a row, so whole sectors move whatever the
 // strides.  Bound by the launch for a decode step (16 rows of 4 x 128: 1.7 us) and by
 // memory for a prompt (4096 such rows, 17 MB: 4.7 us, 3.6 TB/s).
 __global__ void __launch_bounds__(256) k_paged_append(PagedArgs a, const uint16_t* k, const uint16_t* v,
                                                       int64_t row_stride, const int32_t* seq, const int32_t* slot,
-                                                      int T) {
+                                                      int T, const int32_t* pos, int max_pos) {
     pdl_begin();
     const int per_head = a.hd / 8, per_row = a.nkv * per_head;  // 16-byte pieces
     const int64_t n = (int64_t)T * per_row * 2;
@@ -26,7 +27,8 @@ __global__ void __launch_bounds__(256) k_paged_append(PagedArgs a, const uint16_
         const bool isv = r >= per_row;
         const int c = isv ? r - per_row : r, head = c / per_head, piece = c - head * per_head;
         const int s = seq[t], j = slot[t];
-        if ((unsigned)s >= (unsigned)a.n_seqs || (unsigned)j >= (unsigned)a.cap) {
+        if ((unsigned)s >= (unsigned)a.n_seqs || (unsigned)j >= (unsigned)a.cap ||
+            (pos && (unsigned)pos[t] >= (unsigned)max_pos)) {
             atomicExch(a.err, kDevBadPos);
             continue;
         }
@@ -323,11 +325,12 @@ __global__ void __cluster_dims__(kEvC, 1, 1) __launch_bounds__(kInPlaceThreads, 
 }  // namespace
 
 cudaError_t launch_paged_append(const PagedArgs& a, const uint16_t* k, const uint16_t* v, int64_t row_stride,
-                                const int32_t* seq, const int32_t* slot, int T, int num_sms, cudaStream_t st) {
+                                const int32_t* seq, const int32_t* slot, int T, const int32_t* pos, int max_pos,
+                                int num_sms, cudaStream_t st) {
     if (T <= 0) return cudaSuccess;
     const int64_t n = (int64_t)T * a.nkv * (a.hd / 8) * 2, want = (n + 255) / 256, most = (int64_t)num_sms * 8;
     const cudaError_t e = launch_pdl(k_paged_append, dim3((unsigned)(want < most ? want : most)), dim3(256), 0, st, a,
-                                     k, v, row_stride, seq, slot, T);
+                                     k, v, row_stride, seq, slot, T, pos, max_pos);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 

@@ -701,7 +701,7 @@ extern "C" int obs_paged_attn_forward(obs_ctx* ctx, int layer, const obs_paged_k
     CU(launch_qk_norm_rope(ctx->a_qkv, T, nq, nkv, hd, L.q_norm, L.k_norm, ctx->cfg.rms_eps, ctx->rope_cs, ac.max_seq,
                            seq, pos, ctx->a_q, krows, vrows, kv->n_seqs, ctx->err_flag, st, 1),
        "q/k norm, rope");
-    rc = obs_paged_append(ctx, kv, krows, vrows, (int64_t)nkv * hd, seq, slot, T, stream);
+    rc = paged_append(ctx, kv, krows, vrows, (int64_t)nkv * hd, seq, slot, T, pos, ac.max_seq, stream);
     if (rc == OBS_OK)
         rc = q_start ? obs_paged_prefill(ctx, kv, ctx->a_q, (int64_t)nq * hd, ctx->a_out, q_start, T, window, n_sink, 0.0f,
                                          stream)

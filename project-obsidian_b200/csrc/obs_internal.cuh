@@ -272,6 +272,9 @@ namespace obs {
 // what append and decode or prefill would refuse, before the first of them is launched
 int paged_check(obs_ctx* ctx, const obs_paged_kv* kv, bool decode, int window, int n_sink, const float* weights,
                 int w_stride);
+// obs_paged_append; pos (optional): rows whose pos[t] lies outside [0, max_pos) are refused too
+int paged_append(obs_ctx* ctx, const obs_paged_kv* kv, const void* k, const void* v, int64_t row_stride,
+                 const int32_t* seq, const int32_t* slot, int T, const int32_t* pos, int max_pos, void* stream);
 
 // ----------------------------------------------------------------- k_gemm.cu
 enum GemmEpi : int { kEpiSwiglu = 0, kEpiBf16 = 1, kEpiF32 = 2 };

@@ -166,8 +166,8 @@ extern "C" int obs_paged_init(obs_ctx* ctx, const obs_paged_config* cfg) {
     return OBS_OK;
 }
 
-extern "C" int obs_paged_append(obs_ctx* ctx, const obs_paged_kv* kv, const void* k, const void* v, int64_t row_stride,
-                                const int32_t* seq, const int32_t* slot, int T, void* stream) {
+int obs::paged_append(obs_ctx* ctx, const obs_paged_kv* kv, const void* k, const void* v, int64_t row_stride,
+                      const int32_t* seq, const int32_t* slot, int T, const int32_t* pos, int max_pos, void* stream) {
     PAGED_BEGIN();
     if (T < 0) return ctx_fail(ctx, OBS_ERR_INVALID, "T < 0");
     if (T == 0) return OBS_OK;
@@ -177,8 +177,13 @@ extern "C" int obs_paged_append(obs_ctx* ctx, const obs_paged_kv* kv, const void
     if (row_stride < (int64_t)a.nkv * a.hd) return ctx_fail(ctx, OBS_ERR_INVALID, "row_stride is smaller than a row");
     return launched(ctx,
                     launch_paged_append(a, reinterpret_cast<const uint16_t*>(k), reinterpret_cast<const uint16_t*>(v),
-                                        row_stride, seq, slot, T, parts.num_sms, as_stream(stream)),
+                                        row_stride, seq, slot, T, pos, max_pos, parts.num_sms, as_stream(stream)),
                     "paged append");
+}
+
+extern "C" int obs_paged_append(obs_ctx* ctx, const obs_paged_kv* kv, const void* k, const void* v, int64_t row_stride,
+                                const int32_t* seq, const int32_t* slot, int T, void* stream) {
+    return paged_append(ctx, kv, k, v, row_stride, seq, slot, T, nullptr, 0, stream);
 }
 
 extern "C" int obs_paged_decode(obs_ctx* ctx, const obs_paged_kv* kv, const void* q, int64_t q_stride, void* out,

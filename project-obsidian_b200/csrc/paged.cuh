@@ -124,7 +124,8 @@ struct PrefillArgs {
 cudaError_t launch_paged_prefill(PrefillArgs p, float* part, int dtype, int num_sms, cudaStream_t st);
 size_t paged_prefill_part_floats(int num_sms);
 cudaError_t launch_paged_append(const PagedArgs& a, const uint16_t* k, const uint16_t* v, int64_t row_stride,
-                                const int32_t* seq, const int32_t* slot, int T, int num_sms, cudaStream_t st);
+                                const int32_t* seq, const int32_t* slot, int T, const int32_t* pos, int max_pos,
+                                int num_sms, cudaStream_t st);
 cudaError_t launch_paged_evict(const PagedArgs& src, const PagedArgs& dst, const float* w, float* w_dst, int w_stride,
                                int budget, int n_sink, int n_recent, int32_t* kept, int32_t* new_len, cudaStream_t st);
 

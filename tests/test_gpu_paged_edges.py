@@ -79,3 +79,41 @@ def test_infinities_of_a_prompt_reach_the_rows_that_see_them(torch_, dtype, head
             o, a = o.where(want == 0, 0.0), a.where(want == 0, 0.0)
         check_out(mine, o, a, sv, c.dtype)
     ctx.close()
+
+
+# ------------------------------------------------------------------ refused tokens
+@pytest.mark.parametrize("prefill", [False, True])
+def test_a_refused_token_leaves_the_cache_as_it_was(torch_, prefill):
+    """A token whose position lies past the RoPE table, with a slot that the cache has: nothing is appended for it,
+    and what the call gives does not depend on what an earlier call left in the context."""
+    import oracle as O
+    from parity_util import dev
+
+    torch = torch_
+    H, nq, nkv, hd, max_seq, page = 2048, 32, 4, 128, 32, 16
+    ctx = obsmoe.MoeContext(obsmoe.MoeShape(H, 256, 16, 4, n_layers=1, max_tokens=8), 0)
+    ctx.attn_init(nq, nkv, hd, max_seq, 1, 1e7)
+    ctx.load_attn(0, O.synth_attn(seed=9, layer=0, H=H, nq=nq, nkv=nkv, hd=hd))
+    ctx.paged_init(nq, nkv, hd, page, max_seqs=2, max_kv_len=64)
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    table = torch.arange(8, dtype=torch.int32, device="cuda").reshape(2, 4)
+    k, v = (torch.full((8, page, nkv, hd), 0.5, dtype=torch.bfloat16, device="cuda") for _ in "kv")
+    kv = obsmoe.PagedKV(k, v, table, i32(4, 4))
+    start = i32(0, 1, 2) if prefill else None
+    x = dev(torch, O.synth_x(70, 0, 2, H))
+    for bad in (max_seq, max_seq + 5, -1, 1 << 30):
+        outs = []
+        for before in (71, 72):  # what the context's scratch holds
+            y = torch.empty((2, H), dtype=torch.int16, device="cuda")
+            ctx.paged_attn_forward(0, kv, dev(torch, O.synth_x(before, 0, 2, H)), y, 2, i32(0, 1), i32(3, 3), i32(3, 3), start)
+            ctx.check_device()
+            k[:, 3], v[:, 3] = 0.25, 0.75
+            ctx.paged_attn_forward(0, kv, x, y, 2, i32(0, 1), i32(3, bad), i32(3, 3), start)
+            with pytest.raises(obsmoe.ObsError, match="outside the KV caches"):
+                ctx.check_device()
+            # sequence 1's slot (page 4) as it was, sequence 0's written
+            assert bool((k[4, 3] == 0.25).all()) and bool((v[4, 3] == 0.75).all())
+            assert not bool((k[0, 3] == 0.25).all()) and not bool((v[0, 3] == 0.75).all())
+            outs.append(y)
+        assert torch.equal(*outs)
+    ctx.close()
