@@ -91,6 +91,7 @@ class PagedView(C.Structure):
 
 
 DTYPE_BF16, DTYPE_F16 = 0, 1
+_PLANS = {}  # one tuple for equal (page_size, n_kv_heads, head_dim, dtype): calls compare them by identity
 _DTYPES = {"bf16": DTYPE_BF16, "f16": DTYPE_F16}
 
 
@@ -116,9 +117,13 @@ class PagedKV:
             raise ValueError("kv_len and block_table have different numbers of sequences")
         if block_table.shape[0] > 1 and block_table.stride(0) < block_table.shape[1]:
             raise ValueError("block_table's rows may not overlap")
+        if not (k.is_cuda and v.is_cuda and block_table.is_cuda and kv_len.is_cuda):
+            raise ValueError("k, v, block_table and kv_len must be on the GPU")
         self.tensors = (k, v, block_table, kv_len)
+        self.i32 = kv_len.dtype
         self.dtype, self.kv_shape = k.dtype, tuple(k.shape[1:])  # kv_shape: page_size, n_kv_heads, head_dim
-        self.plan = (*self.kv_shape, "bf16" if "bfloat16" in str(k.dtype) else "f16")
+        plan = (*self.kv_shape, "bf16" if "bfloat16" in str(k.dtype) else "f16")
+        self.plan = _PLANS.setdefault(plan, plan)
         self.n_seqs = block_table.shape[0]
         self.view = PagedView(k.data_ptr(), v.data_ptr(), block_table.data_ptr(), kv_len.data_ptr(),
                               k.stride(0), k.stride(1), k.stride(2), self.n_seqs, k.shape[0],
@@ -319,13 +324,15 @@ class MoeContext:
             raise ValueError(f"dtype must be one of {sorted(_DTYPES)}")
         pc = PagedConfig(n_heads, n_kv_heads, head_dim, page_size, max_seqs, max_kv_len, _DTYPES[dtype], int(weights))
         self._chk(lib().obs_paged_init(self._h, C.byref(pc)))
-        self._paged = (page_size, n_kv_heads, head_dim, dtype)
+        plan = (page_size, n_kv_heads, head_dim, dtype)
+        self._paged = _PLANS.setdefault(plan, plan)
         self._paged_row, self._paged_kv_row = n_heads * head_dim, n_kv_heads * head_dim
 
     _paged = None  # page_size, n_kv_heads, head_dim, dtype after paged_init
+    _paged_kv_row = 0
 
     def _paged_kv(self, kv):
-        if kv.plan != self._paged and self._paged is not None:
+        if kv.plan is not self._paged and self._paged is not None:
             raise ValueError(f"the cache's pages are {kv.plan}, the context's {self._paged}")
         return kv.ref
 
@@ -334,39 +341,54 @@ class MoeContext:
         if self._paged is None:  # (the library says what is missing)
             return 0
         row = self._paged_row
-        if q.dtype is not kv.dtype or out.dtype is not kv.dtype:
-            raise ValueError(f"q and out must hold {kv.dtype} like the cache")
+        if q.dtype is not kv.dtype or out.dtype is not kv.dtype or not q.is_cuda or not out.is_cuda:
+            raise ValueError(f"q and out must hold {kv.dtype} like the cache, on the GPU")
         if q.numel() != rows * row or out.numel() != rows * row:
             raise ValueError(f"q and out must be [{rows}, {row}]")
         if not out.is_contiguous():
             raise ValueError("out must be consecutive")
         if q.is_contiguous():
             return row
-        if rows and not q[0].is_contiguous():
+        if q.shape[0] != rows or (rows and not q[0].is_contiguous()):
             raise ValueError("each row of q must be consecutive")
         return q.stride(0) if rows > 1 else row
+
+    @staticmethod
+    def _paged_i32(kv, name, t, least):
+        """The address of `least` consecutive int32 on the GPU (an int is an address, None stays)."""
+        if t is None or t.__class__ is int:
+            return t
+        if t.numel() < least or not t.is_contiguous() or not t.is_cuda \
+                or (t.dtype is not kv.i32 and (t.element_size() != 4 or t.is_floating_point())):
+            raise ValueError(f"{name}: {least} consecutive int32 on the GPU")
+        return t.data_ptr()
 
     def _paged_w(self, kv, w):
         if w is None:
             return None, 0
         if w.dim() != 3 or w.shape[0] != kv.n_seqs or w.shape[1] != kv.kv_shape[1] or w.element_size() != 4 \
-                or not w.is_floating_point() or not w.is_contiguous():
-            raise ValueError("weights: consecutive fp32 [n_seqs, n_kv_heads, positions]")
+                or not w.is_floating_point() or not w.is_contiguous() or not w.is_cuda:
+            raise ValueError("weights: consecutive fp32 [n_seqs, n_kv_heads, positions] on the GPU")
         return w.data_ptr(), w.shape[2]
 
     def paged_append(self, kv, k, v, seq, slot, T, stream=None):
         """Rows k, v [T, n_kv_heads, head_dim] to positions slot[t] of sequences seq[t]."""
         ref = self._paged_kv(kv)
-        row = self._paged_kv_row if self._paged else 0
-        if k.dtype is not kv.dtype or v.dtype is not kv.dtype or k.numel() < T * row or v.numel() < T * row:
-            raise ValueError(f"k and v must be [T, {row}] of {kv.dtype}")
-        stride = row
-        if T and not (k.is_contiguous() and v.is_contiguous()):
-            if not k[0].is_contiguous() or not v[0].is_contiguous() or (T > 1 and k.stride(0) != v.stride(0)):
+        stride = row = self._paged_kv_row
+        if k.dtype is not kv.dtype or v.dtype is not kv.dtype or k.numel() < T * row or v.numel() < T * row \
+                or not k.is_cuda or not v.is_cuda:
+            raise ValueError(f"k and v must be [T, {row}] of {kv.dtype} on the GPU")
+        if not (k.is_contiguous() and v.is_contiguous()) and T:
+            if k.shape[0] < T or v.shape[0] < T or not k[0].is_contiguous() or not v[0].is_contiguous() \
+                    or (T > 1 and k.stride(0) != v.stride(0)):
                 raise ValueError("each row of k and v must be consecutive, their strides the same")
             stride = k.stride(0) if T > 1 else row
-        self._chk((_LIB or lib()).obs_paged_append(self._h, ref, k.data_ptr(), v.data_ptr(), stride, _ptr(seq),
-                                                   _ptr(slot), T, _stream(stream)))
+        # (a decode step's append takes less time on the GPU than here: no calls that it can do without)
+        rc = (_LIB or lib()).obs_paged_append(self._h, ref, k.data_ptr(), v.data_ptr(), stride,
+                                              self._paged_i32(kv, "seq", seq, T), self._paged_i32(kv, "slot", slot, T), T,
+                                              stream if stream is None else _stream(stream))
+        if rc:
+            self._chk(rc)
 
     def paged_decode(self, kv, q, out, window=0, n_sink=0, scale=0.0, weights=None, stream=None):
         """Attention of each sequence's last position over its pages; weights (optional) += the probabilities."""
@@ -379,8 +401,8 @@ class MoeContext:
         """Attention of the sequences' last positions, rows q_start[s] .. q_start[s+1] of q each."""
         ref = self._paged_kv(kv)
         self._chk((_LIB or lib()).obs_paged_prefill(self._h, ref, q.data_ptr(), self._paged_q(kv, q, out, T),
-                                                    out.data_ptr(), _ptr(q_start), T, window, n_sink, scale,
-                                                    _stream(stream)))
+                                                    out.data_ptr(), self._paged_i32(kv, "q_start", q_start, kv.n_seqs + 1),
+                                                    T, window, n_sink, scale, _stream(stream)))
 
     def paged_evict(self, kv, dst, weights, weights_dst, budget, n_sink=0, n_recent=0, kept=None, new_len=None,
                     stream=None):
@@ -391,17 +413,22 @@ class MoeContext:
         wd, wds = self._paged_w(kv, weights_dst)
         if wd is not None and wds != ws:
             raise ValueError("weights and weights_dst must have one shape")
-        if kept is not None and kept.numel() < kv.n_seqs * kv.kv_shape[1] * budget:
-            raise ValueError("kept: int32 [n_seqs, n_kv_heads, budget]")
-        self._chk(lib().obs_paged_evict(self._h, ref, to, w, wd, ws, budget, n_sink, n_recent, _ptr(kept),
-                                        _ptr(new_len), _stream(stream)))
+        self._chk(lib().obs_paged_evict(self._h, ref, to, w, wd, ws, budget, n_sink, n_recent,
+                                        self._paged_i32(kv, "kept", kept, kv.n_seqs * kv.kv_shape[1] * budget),
+                                        self._paged_i32(kv, "new_len", new_len, kv.n_seqs), _stream(stream)))
 
     def paged_attn_forward(self, layer, kv, x, out, T, seq, pos, slot, q_start=None, window=0, n_sink=0, weights=None,
                            stream=None):
         """attn_forward over a paged cache: a decode step (q_start None) or prompts' new tokens."""
         w, ws = self._paged_w(kv, weights)
-        self._chk(lib().obs_paged_attn_forward(self._h, layer, self._paged_kv(kv), _ptr(x), _ptr(out), T, _ptr(seq),
-                                               _ptr(pos), _ptr(slot), _ptr(q_start), window, n_sink, w, ws,
+        for t in (x, out):
+            if t is not None and not isinstance(t, int) and (t.element_size() != 2 or t.numel() < T * self.shape.hidden
+                                                             or not t.is_contiguous() or not t.is_cuda):
+                raise ValueError(f"x and out must be consecutive bf16 [T, {self.shape.hidden}] on the GPU")
+        self._chk(lib().obs_paged_attn_forward(self._h, layer, self._paged_kv(kv), _ptr(x), _ptr(out), T,
+                                               self._paged_i32(kv, "seq", seq, T), self._paged_i32(kv, "pos", pos, T),
+                                               self._paged_i32(kv, "slot", slot, T),
+                                               self._paged_i32(kv, "q_start", q_start, kv.n_seqs + 1), window, n_sink, w, ws,
                                                _stream(stream)))
 
     def synth_layer(self, layer: int, seed: int = 0):
