@@ -117,3 +117,103 @@ def test_a_refused_token_leaves_the_cache_as_it_was(torch_, prefill):
             outs.append(y)
         assert torch.equal(*outs)
     ctx.close()
+
+
+# ------------------------------------------- more sequences than a warp has lanes
+MANY = [
+    # heads, kv, hd, page, sequences, window, sinks
+    (8, 2, 64, 16, 33, 0, 0),
+    (32, 4, 128, 64, 40, 0, 0),
+    (6, 2, 128, 16, 600, 0, 0),       # several sequences per thread of the search
+    (8, 1, 64, 16, 1100, 20, 3),
+]
+
+
+def many(torch, case):
+    """Lengths and new rows of many short sequences: some without rows, some without positions, some with a history."""
+    rng = np.random.default_rng(case)
+    n = MANY[case][4]
+    rows = rng.integers(0, 40, n)
+    rows[::7] = 0
+    rows[n // 2] = 90
+    lens = rows + rng.integers(0, 60, n) * (rng.random(n) < 0.5)
+    lens[3] = 0 if rows[3] == 0 else lens[3]
+    return [int(x) for x in lens], [int(x) for x in rows]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("case", range(len(MANY)))
+def test_prefill_of_many_sequences(torch_, dtype, case):
+    from paged_util import Cache
+    from test_gpu_paged import check_prefill
+
+    heads, kv, hd, page, n, window, sinks = MANY[case]
+    lens, rows = many(torch_, case)
+    c = Cache(lens, kv, hd, page, dtype, seed=120 + case)
+    ctx = make_ctx(heads, kv, hd, page, dtype, seqs=n)
+    check_prefill(torch_, c, ctx, heads, rows, window, sinks, 120 + case)
+    ctx.close()
+
+
+def test_prefill_of_many_sequences_with_one_row_each(torch_):
+    """As many rows as sequences and few of them: the split form, 40 sequences."""
+    from paged_util import Cache
+    from test_gpu_paged import check_prefill
+
+    c = Cache([1 + 37 * i for i in range(40)], 1, 128, 16, "bf16", seed=130)
+    ctx = make_ctx(8, 1, 128, 16, seqs=40)
+    check_prefill(torch_, c, ctx, 8, [1] * 40, 0, 0, 130)
+    ctx.close()
+
+
+def test_prefill_of_many_sequences_refuses_bad_row_ranges(torch_):
+    from paged_util import Cache
+    from test_gpu_paged import check_prefill
+
+    torch = torch_
+    n = 40
+    c = Cache([9] * n, 2, 64, 16, "bf16", seed=131)
+    ctx = make_ctx(8, 2, 64, 16, seqs=n)
+    q = queries(torch, 2 * n, 8, 64, c.dtype, 131)
+    out = torch.empty_like(q)
+    good = torch.arange(0, 2 * n + 1, 2, dtype=torch.int32)
+    for at, x in ((0, 1), (0, -2), (n, 2 * n - 1), (n, 2 * n + 3), (n // 2, 0), (n // 2, 1 << 30), (35, -5)):
+        bad = good.clone()
+        bad[at] = x
+        ctx.paged_prefill(view(c), q, out, bad.cuda(), 2 * n)
+        with pytest.raises(obsmoe.ObsError, match="outside the KV caches"):
+            ctx.check_device()
+    check_prefill(torch, c, ctx, 8, [2] * n, 0, 0, 131)
+    ctx.close()
+
+
+# ----------------------------------- eviction past what a cluster's shared memory holds
+@pytest.mark.parametrize("kind", ["plain", "ties", "odd", "same"])
+@pytest.mark.parametrize("lens,budget,sinks,recent", [([70000, 65540, 66000], 30000, 4, 500), ([140000, 9000], 20001, 0, 0),
+                                                      ([300001], 299990, 3, 1000)])
+def test_evict_long_caches(torch_, kind, lens, budget, sinks, recent):
+    from paged_util import Cache
+    from test_gpu_paged import check_evicted, weights_of
+
+    torch = torch_
+    kv, hd, page, n = 1, 8, 64, len(lens)
+    c = Cache(lens, kv, hd, page, "bf16", seed=140)
+    ctx = make_ctx(4, kv, hd, page, max_len=max(lens))
+    w = weights_of(torch, kind, (n, kv, max(lens)), 140)
+    before = [tuple(x.clone() for x in c.rows(s, ln)) for s, ln in enumerate(lens)]
+    per = -(-budget // page)
+    to_table = torch.randperm(n * per, device="cuda").to(torch.int32).reshape(n, per)
+    to_k, to_v = (torch.zeros((n * per, page, kv, hd), dtype=c.dtype, device="cuda") for _ in range(2))
+    kept, kept2 = (torch.full((n, kv, budget), 77, dtype=torch.int32, device="cuda") for _ in range(2))
+    new_len, len2 = (torch.full((n,), 77, dtype=torch.int32, device="cuda") for _ in range(2))
+    w_dst = torch.full_like(w, 9.0)
+    ctx.paged_evict(view(c), obsmoe.PagedKV(to_k, to_v, to_table, new_len), w, w_dst, budget, n_sink=sinks, n_recent=recent,
+                    kept=kept, new_len=new_len)
+    ctx.check_device()
+    check_evicted(torch, c, before, w, kept, new_len, budget, sinks, recent, to_k, to_v, to_table, w_dst)
+    w2 = w.clone()
+    ctx.paged_evict(view(c), view(c), w2, w2, budget, n_sink=sinks, n_recent=recent, kept=kept2, new_len=len2)
+    ctx.check_device()
+    assert torch.equal(kept, kept2) and torch.equal(new_len, len2)
+    check_evicted(torch, c, before, w, kept2, len2, budget, sinks, recent, c.k, c.v, c.table, w2)
+    ctx.close()
