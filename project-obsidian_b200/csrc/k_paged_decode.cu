@@ -35,8 +35,8 @@
 // is common: p <= 1 is multiplied by 2^15 there, and the sums by 2^-15 at their end.
 //
 // An infinity in V times what rounding left of its p, zero or negative, would be NaN: a
-// head whose sums are not finite although its l is takes its positions again one by one
-// (attend_row).  When nothing is wrong this costs a comparison.
+// CTA whose sums of a run are not finite although l is computes those of its run again
+// (attend_again), before the join.  When nothing is wrong this costs a comparison.
 //
 // Measured, 32 / 4 heads of 128: 32 sequences of 61 to 32768 positions in f16, pages of
 // 16: 172 us, 6.5 TB/s, 97% of the measured copy rate; 128 sequences with a window of
@@ -71,18 +71,6 @@ __device__ __forceinline__ uint32_t movm(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-template <int DT>
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (DT == 0)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
 // The visible tiles of one sequence: tiles 0 .. ts-1 (sinks), then wt .. (window).
 struct Span {
     int n, lo, sink_end;  // positions held, the window's first, the sinks' end
@@ -123,22 +111,26 @@ __device__ __forceinline__ bool needs_again(const float (&o)[4], float l) {
     const float z = o[0] * 0.0f + o[1] * 0.0f + (o[2] * 0.0f + o[3] * 0.0f);  // NaN unless all are finite
     return z != 0.0f && l > 0.0f && l <= 3.4e38f;
 }
-// One head once more, by a warp.
-template <int DT>
-__device__ __forceinline__ void again(const DecodeArgs& p, int s, int h, int head, int sink_end, int lo, int n) {
-    using X = Elem<DT>;
+// The group's rows of one run again, by a warp for 64 dimensions: tiles x0 .. x1 of (s, h),
+// `part` null where the run is all of it.  run: each head's maximum and sum.
+template <int DT, int HD>
+__device__ __noinline__ void run_again(const DecodeArgs& p, int s, int h, int x0, int x1, float* part, const float2* run) {
     const PagedArgs& a = p.c;
-    const int lane = threadIdx.x & 31;
-    const int64_t at = (h * a.group + head) * a.hd + 4 * lane;
-    float qf[4] = {0.0f, 0.0f, 0.0f, 0.0f}, acc[4], m, l;
-    if (4 * lane < a.hd) {
-        const uint2 w = *reinterpret_cast<const uint2*>(p.q + s * p.q_stride + at);
-        qf[0] = X::lo(w.x), qf[1] = X::hi(w.x), qf[2] = X::lo(w.y), qf[3] = X::hi(w.y);
+    const int g = (threadIdx.x & 31) >> 2, warp = threadIdx.x >> 5, nq = a.nkv * a.group;
+    if (warp >= HD / 64) return;
+    const Span sp = span_of(seq_len(a, s), p.window, p.n_sink);
+    AgainRows rows;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const int head = g + 8 * r;
+        const bool in = head < a.group;
+        rows.q[r] = in ? p.q + s * p.q_stride + (h * a.group + head) * a.hd : nullptr;
+        rows.out[r] = part ? static_cast<void*>(part + head * HD)
+                           : static_cast<void*>(p.out + ((int64_t)s * nq + h * a.group + head) * a.hd);
+        rows.i[r] = sp.n - 1, rows.lo[r] = sp.lo;
+        rows.ref[r] = in ? run[head].x : 0.0f, rows.l[r] = in ? run[head].y : 1.0f;
     }
-    attend_row<DT>(a, s, h, qf, p.scale, sink_end, lo, n, acc, m, l);
-    if (4 * lane < a.hd)
-        *reinterpret_cast<uint2*>(p.out + (int64_t)s * a.nkv * a.group * a.hd + at) =
-            make_uint2(X::pack(acc[0] / l, acc[1] / l), X::pack(acc[2] / l, acc[3] / l));
+    attend_again<DT>(a, s, h, rows, part != nullptr, x0, x1 - x0 + 1, sp.ts, sp.wt, p.n_sink, p.scale_log2, warp);
 }
 
 template <int HD>
@@ -152,7 +144,7 @@ struct DecodeSmem {
 };
 
 template <int DT, int HD, int NT>
-__global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
+__global__ void __launch_bounds__(kThreads, 2) k_paged_decode(const __grid_constant__ DecodeArgs p) {
     pdl_begin();
     using X = Elem<DT>;
     using M = DecodeSmem<HD>;
@@ -160,6 +152,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     float* s_mrg = reinterpret_cast<float*>(smem + M::RING);
     __shared__ float s_m[kWarps][16], s_l[kWarps][16];
+    __shared__ float2 s_run[16];  // the run's maximum (0 for -inf) and sum
     __shared__ uint32_t s_scan[kWarps], s_first;
     __shared__ int s_seq;
     __shared__ int s_last;
@@ -414,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
             }
         __syncthreads();
         const int hsub = tid >> 4, dsub = (tid & 15) * 4;  // of 8 heads x 64 dimensions
-        uint32_t bad = 0;  // heads this thread has written a sum of that is not finite, with l > 0 that is
+        bool bad = false;  // a sum of this thread's is not finite, with l > 0 that is
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int head = nt * 8 + hsub;
@@ -445,12 +438,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
                         o[0] += mw[w] * v.x, o[1] += mw[w] * v.y, o[2] += mw[w] * v.z, o[3] += mw[w] * v.w;
                     }
                     const int d = half * 64 + dsub;
+                    bad |= needs_again(o, ls);
                     if (whole) {
                         if (d < a.hd) {
                             uint16_t* dst = p.out + ((int64_t)cs.s * nq + cs.h * G + head) * a.hd + d;
                             *reinterpret_cast<uint2*>(dst) =
                                 make_uint2(X::pack(o[0] / ls, o[1] / ls), X::pack(o[2] / ls, o[3] / ls));
-                            bad |= (uint32_t)needs_again(o, ls) << head;
                         }
                     } else {
                         *reinterpret_cast<float4*>(part + head * HD + d) = make_float4(o[0], o[1], o[2], o[3]);
@@ -458,6 +451,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
                 }
             }
             if (head < G && (tid & 15) == 0) {
+                s_run[head] = make_float2(ref, ls);
                 if (whole) {
                     if (p.ml) p.ml[(int64_t)cs.s * nq + cs.h * G + head] = make_float2(ref, ls);
                 } else {
@@ -465,11 +459,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
                 }
             }
         }
+        if (__syncthreads_or(bad)) {
+            run_again<DT, HD>(p, cs.s, cs.h, x_first, cs.x, whole ? nullptr : part, s_run);
+            __syncthreads();
+        }
         if (!whole) {
             // ---- the last CTA of the item joins its parts, in their order
             const int c0 = (int)owner_of(first_u), c1 = (int)owner_of(last_u);
             const int parts = c1 - c0 + 1;
-            __syncthreads();
             if (tid == 0) {
                 __threadfence();
                 s_last = atomicInc(p.count + c0, parts - 1) == (unsigned)(parts - 1);
@@ -530,19 +527,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(DecodeArgs p) {
                         uint16_t* dst = p.out + ((int64_t)cs.s * nq + cs.h * G + head) * a.hd + d;
                         *reinterpret_cast<uint2*>(dst) = make_uint2(X::pack(o[r][0] / L[r], o[r][1] / L[r]),
                                                                     X::pack(o[r][2] / L[r], o[r][3] / L[r]));
-                        bad |= (uint32_t)needs_again(o[r], L[r]) << head;
                         if (p.ml && d == 0)
                             p.ml[(int64_t)cs.s * nq + cs.h * G + head] = make_float2(M[r] == -INFINITY ? 0.0f : M[r], L[r]);
                     }
                 }
             }
-        }
-        bad = __reduce_or_sync(0xffffffffu, bad);  // (a warp writes all of a head)
-        __syncwarp();  // the head's first values before the second, which other lanes store
-        while (bad) {
-            const int head = __ffs(bad) - 1;
-            bad &= bad - 1;
-            again<DT>(p, cs.s, cs.h, head, cs.sp.sink_end, cs.sp.lo, cs.sp.n);
         }
         __syncthreads();  // s_m, s_l and s_mrg are written again by the next run
         fresh = true;

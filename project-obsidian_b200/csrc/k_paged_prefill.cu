@@ -57,8 +57,8 @@
 // grown by), and so are l and O.
 //
 // A NaN or infinity in V meets p = 0 of rows that do not see it, and 0 * NaN is NaN:
-// a row whose result is not finite is computed again from its visible positions
-// alone (attend_row), unless l says that its own scores are the reason (NaN or +inf
+// a row whose sums are not finite has those computed again from its visible positions
+// alone (attend_again), unless l says that its own scores are the reason (NaN or +inf
 // among them, or all -inf: the whole row is NaN).  When nothing is wrong this costs a
 // comparison.
 //
@@ -203,32 +203,48 @@ __device__ __forceinline__ int row_of(const PagedArgs& a, uint32_t magic, int q0
     return h * a.group + g;
 }
 
-template <int DT>
-__device__ __forceinline__ void recompute_row(const PrefillArgs& p, int s, int h, int64_t t, int head, int i) {
-    using X = Elem<DT>;
+// A block's rows that are computed again: 16 w .. 16 w + 15 by warp w, against the CTA's tiles.
+struct Again {
+    int any, s, q0, base, R0, x0, nt, ts, wt;
+    uint32_t rows[kRows / 32];  // which
+};
+// Each warp's rows: ref and l, p = 2^(x - ref) / l, at its staging place (stg).
+template <int DT, int HD>
+__device__ __forceinline__ void rows_again(const PrefillArgs& p, const Again& b, const uint8_t* smem) {
     const PagedArgs& a = p.c;
-    const int lane = threadIdx.x & 31;
-    const uint16_t* q = p.q + t * p.q_stride + head * a.hd;
-    float qf[4] = {0.0f, 0.0f, 0.0f, 0.0f}, acc[4], m, l;
-    if (4 * lane < a.hd) {
-        const uint2 w = *reinterpret_cast<const uint2*>(q + 4 * lane);
-        qf[0] = X::lo(w.x), qf[1] = X::hi(w.x), qf[2] = X::lo(w.y), qf[3] = X::hi(w.y);
+    const int lane = threadIdx.x & 31, r0 = (threadIdx.x >> 5) * 16, nq = a.nkv * a.group, h = blockIdx.x % a.nkv;
+    const uint32_t which = b.rows[r0 / 32] >> (r0 & 16) & 0xFFFFu;
+    if (!which) return;
+    const float2* ref_l = reinterpret_cast<const float2*>(smem + r0 / kM * Pf<HD>::QTILE + (r0 / 32 & 3) * 4096) + (r0 & 16);
+    const bool split = p.splits > 1;
+    AgainRows rows;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int r = (lane >> 2) + 8 * k;
+        int t;
+        const int head = row_of(a, p.group_magic, b.q0, h, b.R0 + r0 + r, &t);
+        const bool in = which >> r & 1u;
+        const int64_t row = (int64_t)t * nq + head;
+        rows.q[k] = in ? p.q + t * p.q_stride + head * a.hd : nullptr;
+        rows.out[k] = split ? static_cast<void*>(p.part_acc + ((int64_t)blockIdx.y * p.T * nq + row) * HD)
+                            : static_cast<void*>(p.out + row * a.hd);
+        rows.i[k] = b.base + (t - b.q0), rows.lo[k] = window_lo(rows.i[k], p.window);
+        rows.ref[k] = in ? ref_l[r].x : 0.0f, rows.l[k] = in ? ref_l[r].y : 1.0f;
     }
-    const int lo = window_lo(i, p.window);
-    attend_row<DT>(a, s, h, qf, p.scale, min(p.n_sink, lo), lo, i + 1, acc, m, l);
-    if (4 * lane < a.hd)
-        *reinterpret_cast<uint2*>(p.out + (t * a.nkv * a.group + head) * a.hd + 4 * lane) =
-            make_uint2(X::pack(acc[0] / l, acc[1] / l), X::pack(acc[2] / l, acc[3] / l));
+#pragma unroll 1
+    for (int v = 0; v < HD / 64; ++v)
+        attend_again<DT>(a, b.s, h, rows, split, b.x0, b.nt, b.ts, b.wt, p.n_sink, p.scale_log2, v);
 }
 
 template <int DT, int HD>
-__global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
+__global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(const __grid_constant__ PrefillArgs p) {
     pdl_begin();
     using X = Elem<DT>;
     using C = Pf<HD>;
     constexpr float kShift = DT == 0 ? 0.0f : 7.0f;  // p is taken against m - kShift
     extern __shared__ uint8_t smem_raw[];
     __shared__ int s_scan[kThreads / 32];
+    __shared__ Again s_again;
     __shared__ int s_blk[5];  // sequence, block of it, its rows' range, its length
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
@@ -350,6 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
     }
     // (nt <= 2^14, splits <= the number of SMs)
     const int x0 = split ? tl.nt * z / ns : 0, nt = (split ? tl.nt * (z + 1) / ns : tl.nt) - x0;
+    if (warp == kWarpMma + 2 && lane == 0) s_again = {0, s, q0, base, R0, x0, nt, tl.ts, tl.wt, {}};
     auto tile_key = [&](int x) { return (x < tl.ts ? x : x - tl.ts + tl.wt) * kKeys; };
     const bool precise = i_lo < 0 || seen(i_lo, p.window, p.n_sink) < kFewKeys;
 
@@ -615,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
         if (ok) {
             tc_fence_after();
             const int64_t row = (int64_t)t * nq + head;
-            float2 fin = make_float2(0.0f, 0.0f);
+            float2 fin = make_float2(0.0f, 0.0f);  // NaN once a sum is not finite
             uint8_t* stg = smem + x * C::QTILE + (warp & 3) * 4096;
             if (split && valid) p.part_ml[(int64_t)z * p.T * nq + row] = make_float2(m - kShift, l);
             const float inv = i < 0 ? 1.0f : 1.0f / l;
@@ -629,23 +646,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
 #pragma unroll
                     for (int e = 0; e < 64; ++e) o[e] = 0.0f;
                 }
+#pragma unroll
+                for (int e = 0; e < 64; e += 2)
+                    fin = fma2(make_float2(o[e], o[e + 1]), make_float2(0.0f, 0.0f), fin);
                 if (split) {
                     float4* dst = reinterpret_cast<float4*>(p.part_acc + ((int64_t)z * p.T * nq + row) * HD + c);
                     if (valid)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                 } else {
-// through shared memory (Q's rows of this warp, which no product needs any more), so
+                    // through shared memory (Q's rows of this warp, which no product needs any more), so
                     // that a store writes whole lines: piece e of row lane lies at e ^ (lane % 8)
                     __syncwarp();
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         float* y = o + 8 * e;
 #pragma unroll
-                        for (int d = 0; d < 8; d += 2) {
-                            fma2(y[d], y[d + 1], inv, 0.0f);
-                            fin = fma2(make_float2(y[d], y[d + 1]), make_float2(0.0f, 0.0f), fin);  // NaN once one is not finite
-                        }
+                        for (int d = 0; d < 8; d += 2) fma2(y[d], y[d + 1], inv, 0.0f);
                         *reinterpret_cast<uint4*>(stg + lane * 128 + ((e ^ (lane & 7)) << 4)) =
                             make_uint4(X::pack(y[0], y[1]), X::pack(y[2], y[3]), X::pack(y[4], y[5]), X::pack(y[6], y[7]));
                     }
@@ -660,13 +677,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
                     }
                 }
             }
-            uint32_t again = __ballot_sync(0xffffffffu, valid && i >= 0 && !(fin.x + fin.y == 0.0f) && l > 0.0f && l <= 3.4e38f && !split);
-            __syncwarp();  // the rows' first values before the second, which other lanes store
-            while (again) {  // (never with split: k_paged_join does it)
-                const int who = __ffs(again) - 1;
-                again &= again - 1;
-                recompute_row<DT>(p, s, h, __shfl_sync(0xffffffffu, t, who), __shfl_sync(0xffffffffu, head, who),
-                                  __shfl_sync(0xffffffffu, i, who));
+            const uint32_t again =
+                __ballot_sync(0xffffffffu, valid && i >= 0 && !(fin.x + fin.y == 0.0f) && l > 0.0f && l <= 3.4e38f);
+            if (again) {
+                reinterpret_cast<float2*>(stg)[lane] = make_float2(m - kShift, l);
+                if (lane == 0) s_again.rows[warp] = again, s_again.any = 1;
             }
         }
     }
@@ -674,6 +689,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(PrefillArgs p) {
     __syncthreads();
     tc_fence_after();
     if (warp == kWarpMma) tmem_dealloc(tmem, 512);
+    if (s_again.any) rows_again<DT, HD>(p, s_again, smem);
     if (tid == 0 && s_abort) {
         atomicExch(a.err + 1, s_abort);
         atomicExch(a.err, kDevTimeout);
@@ -729,20 +745,14 @@ __global__ void __launch_bounds__(256) k_paged_join(PrefillArgs p) {
             }
         }
     }
-    bool bad = false;
 #pragma unroll
-    for (int e = 0; e < PER; ++e) {
-        o[e] = i < 0 ? 0.0f : o[e] / l;
-        bad |= !(fabsf(o[e]) <= 3.4e38f) && l > 0.0f && l <= 3.4e38f;
-    }
+    for (int e = 0; e < PER; ++e) o[e] = i < 0 ? 0.0f : o[e] / l;
     const int d = lane * PER;
     if (d < a.hd) {
         uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + row * a.hd + d);
         if constexpr (PER == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(X::pack(o[0], o[1]), X::pack(o[2], o[3]));
         else *dst = X::pack(o[0], o[1]);
     }
-    __syncwarp();
-    if (__any_sync(0xffffffffu, bad)) recompute_row<DT>(p, s, head / a.group, t, head, i);
 }
 
 template <int DT, int HD>

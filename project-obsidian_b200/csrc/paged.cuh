@@ -162,37 +162,194 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
 }
 
-// One query row against its visible positions, one warp, scalar (lane l holds the
-// four dimensions 4l .. 4l+3): the online softmax in the order of the positions.
-// qf: the lane's four query values; acc, m, l: the lane's four output sums, the
-// maximum and the sum.  Positions are visited as [0, sink_end) then [lo, hi).
 template <int DT>
-__device__ __forceinline__ void attend_row(const PagedArgs& a, int s, int head, const float (&qf)[4], float scale,
-                                           int sink_end, int lo, int hi, float (&acc)[4], float& m, float& l) {
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (DT == 0)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// ---- rows whose result is not finite although the sum of their exponentials is: a NaN
+// or an infinity in V, which the products spread to rows that do not see it (0 * NaN) and
+// turn into NaN (infinity times what rounding left of p).  Their dimensions that are not
+// finite are computed again, 16 rows by a warp: p from the known maximum and sum, the
+// products on mma.sync with the positions that hold anything not finite taken out, and
+// those, for the rows that see them, by fp32 FMAs, where IEEE arithmetic does what the
+// formula says.
+//
+// Bounded: every position that the rows see is read once more per 16 rows, whatever V
+// holds.  One prompt of 4096 (32 / 4 heads of 128, bf16) with one infinity at its front,
+// which every row sees: 1.9 ms; with nothing but infinities in V 8.9 ms; 155 us without.
+// A row by a warp, one position at a time, took 25 ms for a prompt of 2048.
+struct AgainRows {              // a lane's two rows: g and g + 8 of 16, g = lane / 4
+    const uint16_t* q[2];       // null: no such row
+    void* out[2];               // 16-bit values, or fp32 (then times l)
+    int i[2], lo[2];            // its position and its window's first
+    float ref[2], l[2];         // p = 2^(scale log2 e q . k - ref) / l
+};
+// Positions: tiles x0 .. x0 + nt of 64 (x < ts: tile x, else x - ts + wt).  Dimensions 64 v .. 64 v + 63.
+template <int DT>
+__device__ __forceinline__ void attend_again(const PagedArgs& a, int s, int h, const AgainRows& rows, bool f32, int x0, int nt,
+                                          int ts, int wt, int n_sink, float scale_log2, int v) {
     using X = Elem<DT>;
-    const int lane = threadIdx.x & 31;
-    const bool mine = 4 * lane < a.hd;
-    m = -INFINITY, l = 0.0f;
+    constexpr uint32_t kExp = DT == 0 ? 0x7F80u : 0x7C00u;
+    constexpr float kScaleP = DT == 0 ? 1.0f : 32768.0f;  // f16 holds nothing below 2^-25
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int hd = a.hd;
+    float wl[2];
+    int i_max = -1, lo_min = 0x7fffffff;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] = 0.0f;
-    for (int j = sink_end > 0 ? 0 : lo; j < hi; j = (j + 1 == sink_end && lo > sink_end) ? lo : j + 1) {
-        const int64_t off = row_offset(a, s, j, head);
-        uint2 kw = make_uint2(0, 0), vw = make_uint2(0, 0);
-        if (mine && off >= 0) {
-            kw = *reinterpret_cast<const uint2*>(a.k + off + 4 * lane);
-            vw = *reinterpret_cast<const uint2*>(a.v + off + 4 * lane);
-        }
-        float x = qf[0] * X::lo(kw.x) + qf[1] * X::hi(kw.x) + qf[2] * X::lo(kw.y) + qf[3] * X::hi(kw.y);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        x *= scale;
-        const float mn = fmaxf(m, x), ref = mn == -INFINITY ? 0.0f : mn;
-        const float corr = expf(m - ref), p = expf(x - ref);
-        l = l * corr + p;
-        acc[0] = acc[0] * corr + p * X::lo(vw.x), acc[1] = acc[1] * corr + p * X::hi(vw.x);
-        acc[2] = acc[2] * corr + p * X::lo(vw.y), acc[3] = acc[3] * corr + p * X::hi(vw.y);
-        m = mn;
+    for (int r = 0; r < 2; ++r) {
+        const bool row = rows.q[r] != nullptr;
+        wl[r] = kScaleP / rows.l[r];
+        if (row) i_max = max(i_max, rows.i[r]), lo_min = min(lo_min, rows.lo[r]);
     }
+    i_max = __reduce_max_sync(0xffffffffu, i_max), lo_min = __reduce_min_sync(0xffffffffu, lo_min);
+    auto sees = [&](int r, int j) {
+        return rows.q[r] != nullptr && j <= rows.i[r] && (j >= rows.lo[r] || j < n_sink);
+    };
+    // acc[e][2 r + b]: row r of the lane's, dimension 64 v + 16 t + 8 b + e
+    float acc[8][4];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[e][c] = 0.0f;
+
+#pragma unroll 1
+    for (int n = 0; n < 4 * nt; ++n) {
+        const int x = x0 + n / 4, j0 = (x < ts ? x : x - ts + wt) * 64 + (n & 3) * 16;
+        int64_t off = -1;
+        const int jl = j0 + (lane & 15);
+        if (jl <= i_max && (jl >= lo_min || jl < n_sink)) off = row_offset(a, s, jl, h);
+        if (!__any_sync(0xffffffffu, off >= 0)) continue;
+        float x8[2][4];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int64_t o = __shfl_sync(0xffffffffu, off, 8 * half + g);
+            float (&c)[4] = x8[half];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[e] = 0.0f;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                // any order of the dimensions will do in q . k, the same for both: lane t takes 16
+                // bytes, dimensions 32 u + 8 t .. + 7, for two steps of 16 (q again for every 8
+                // positions: held, it would cost the calling kernel's loop registers)
+                uint4 k = make_uint4(0, 0, 0, 0), q0 = k, q1 = k;
+                const int d = 32 * u + 8 * t;
+                if (d < hd) {
+                    if (o >= 0) k = *reinterpret_cast<const uint4*>(a.k + o + d);
+                    if (rows.q[0]) q0 = *reinterpret_cast<const uint4*>(rows.q[0] + d);
+                    if (rows.q[1]) q1 = *reinterpret_cast<const uint4*>(rows.q[1] + d);
+                }
+                const uint32_t a0[4] = {q0.x, q1.x, q0.y, q1.y}, a1[4] = {q0.z, q1.z, q0.w, q1.w};
+                mma16816<DT>(c, a0, k.x, k.y);
+                mma16816<DT>(c, a1, k.z, k.w);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {  // row e / 2 of the lane's, position 2 t + e % 2
+                c[e] = sees(e >> 1, j0 + 8 * half + 2 * t + (e & 1)) ? ex2(c[e] * scale_log2 - rows.ref[e >> 1]) * wl[e >> 1] : 0.0f;
+            }
+        }
+        // p and what its rounding left, as the A operand of 16 positions
+        uint32_t p[4], rest[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float p0 = x8[e >> 1][2 * (e & 1)], p1 = x8[e >> 1][2 * (e & 1) + 1];
+            p[e] = X::pack(p0, p1);
+            rest[e] = X::pack(p0 - X::lo(p[e]), p1 - X::hi(p[e]));
+        }
+        // rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of V, dimensions 64 v + 8 g .. + 7
+        uint4 w[4];
+        uint32_t odd = 0;  // bit r: the lane's piece of row r holds something not finite
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int64_t o = __shfl_sync(0xffffffffu, off, 2 * t + (r & 1) + 8 * (r >> 1));
+            w[r] = make_uint4(0, 0, 0, 0);
+            if (o >= 0 && 64 * v + 8 * g < hd) w[r] = *reinterpret_cast<const uint4*>(a.v + o + 64 * v + 8 * g);
+            const uint32_t z[4] = {w[r].x, w[r].y, w[r].z, w[r].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if ((z[e] & kExp) == kExp || (z[e] >> 16 & kExp) == kExp) odd |= 1u << r;
+        }
+        uint32_t taken = 0;  // positions of the 16 that hold something not finite
+        if (__any_sync(0xffffffffu, odd != 0)) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t who = __ballot_sync(0xffffffffu, odd >> r & 1u);  // lanes 4 g + t
+#pragma unroll
+                for (int tt = 0; tt < 4; ++tt)
+                    if (who >> tt & 0x11111111u) taken |= 1u << (2 * tt + (r & 1) + 8 * (r >> 1));
+                if (taken >> (2 * t + (r & 1) + 8 * (r >> 1)) & 1u) w[r] = make_uint4(0, 0, 0, 0);
+            }
+        }
+        // column g of the product e is dimension 64 v + 8 g + e
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int sel = e & 1 ? 0x7632 : 0x5410;
+            const uint32_t lo4[4] = {w[0].x, w[0].y, w[0].z, w[0].w}, lo5[4] = {w[1].x, w[1].y, w[1].z, w[1].w};
+            const uint32_t hi4[4] = {w[2].x, w[2].y, w[2].z, w[2].w}, hi5[4] = {w[3].x, w[3].y, w[3].z, w[3].w};
+            const uint32_t b0 = __byte_perm(lo4[e >> 1], lo5[e >> 1], sel), b1 = __byte_perm(hi4[e >> 1], hi5[e >> 1], sel);
+            mma16816<DT>(acc[e], rest, b0, b1);
+            mma16816<DT>(acc[e], p, b0, b1);
+        }
+        while (taken) {
+            const int c = __ffs(taken) - 1;
+            taken &= taken - 1;
+            const int64_t o = __shfl_sync(0xffffffffu, off, c);
+            const int half = c >> 3, from = (lane & ~3) | ((c & 7) >> 1);  // the lane that holds the rows' p at c
+            float pc[2];
+            bool see[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float p0 = __shfl_sync(0xffffffffu, half ? x8[1][2 * r] : x8[0][2 * r], from);
+                const float p1 = __shfl_sync(0xffffffffu, half ? x8[1][2 * r + 1] : x8[0][2 * r + 1], from);
+                pc[r] = c & 1 ? p1 : p0, see[r] = sees(r, j0 + c);
+            }
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const int d = 64 * v + 16 * t + 8 * b;
+                if (o < 0 || d >= hd) continue;
+                const uint4 y = *reinterpret_cast<const uint4*>(a.v + o + d);
+                const uint32_t z[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float f = e & 1 ? X::hi(z[e >> 1]) : X::lo(z[e >> 1]);
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+                        if (see[r]) acc[e][2 * r + b] += pc[r] * f;
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int d = 64 * v + 16 * t + 8 * b;
+            if (rows.q[r] == nullptr || d >= hd) continue;
+            if (f32) {
+                float* dst = static_cast<float*>(rows.out[r]) + d;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (!(fabsf(dst[e]) <= 3.4e38f)) dst[e] = acc[e][2 * r + b] / wl[r];
+            } else {
+                uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(rows.out[r]) + d);
+                const uint4 y = *dst;
+                uint32_t z[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t n = X::pack(acc[2 * e][2 * r + b] * (1.0f / kScaleP), acc[2 * e + 1][2 * r + b] * (1.0f / kScaleP));
+                    if ((z[e] & kExp) == kExp) z[e] = (z[e] & 0xFFFF0000u) | (n & 0xFFFFu);
+                    if ((z[e] >> 16 & kExp) == kExp) z[e] = (z[e] & 0xFFFFu) | (n & 0xFFFF0000u);
+                }
+                *dst = make_uint4(z[0], z[1], z[2], z[3]);
+            }
+        }
 }
 
 }  // namespace obs
