@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(const __grid_const
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
                 mw[w] = ex2(s_m[w][head] - ref), ls += mw[w] * s_l[w][head];
-                mw[w] *= 1.0f / kScaleP;  // of the sums of p v
+                mw[w] *= whole ? 1.0f / kScaleP : kJoinScale / kScaleP;  // of the sums of p v
             }
 #pragma unroll
             for (int half = 0; half < HD / 64; ++half) {
@@ -455,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(const __grid_const
                 if (whole) {
                     if (p.ml) p.ml[(int64_t)cs.s * nq + cs.h * G + head] = make_float2(ref, ls);
                 } else {
-                    reinterpret_cast<float2*>(part + G * HD)[head] = make_float2(mx, ls);
+                    reinterpret_cast<float2*>(part + G * HD)[head] = make_float2(mx, ls * kJoinScale);
                 }
             }
         }
@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_decode(const __grid_const
                         *reinterpret_cast<uint2*>(dst) = make_uint2(X::pack(o[r][0] / L[r], o[r][1] / L[r]),
                                                                     X::pack(o[r][2] / L[r], o[r][3] / L[r]));
                         if (p.ml && d == 0)
-                            p.ml[(int64_t)cs.s * nq + cs.h * G + head] = make_float2(M[r] == -INFINITY ? 0.0f : M[r], L[r]);
+                            p.ml[(int64_t)cs.s * nq + cs.h * G + head] = make_float2(M[r] == -INFINITY ? 0.0f : M[r], L[r] / kJoinScale);
                     }
                 }
             }

@@ -634,8 +634,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(const __grid_cons
             const int64_t row = (int64_t)t * nq + head;
             float2 fin = make_float2(0.0f, 0.0f);  // NaN once a sum is not finite
             uint8_t* stg = smem + x * C::QTILE + (warp & 3) * 4096;
-            if (split && valid) p.part_ml[(int64_t)z * p.T * nq + row] = make_float2(m - kShift, l);
-            const float inv = i < 0 ? 1.0f : 1.0f / l;
+            if (split && valid) p.part_ml[(int64_t)z * p.T * nq + row] = make_float2(m - kShift, l * kJoinScale);
+            const float inv = split ? kJoinScale : i < 0 ? 1.0f : 1.0f / l;
 #pragma unroll
             for (int c = 0; c < HD; c += 64) {
                 float o[64];
@@ -653,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_prefill(const __grid_cons
                     float4* dst = reinterpret_cast<float4*>(p.part_acc + ((int64_t)z * p.T * nq + row) * HD + c);
                     if (valid)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                        for (int e = 0; e < 16; ++e) dst[e] = make_float4(o[4 * e] * inv, o[4 * e + 1] * inv, o[4 * e + 2] * inv, o[4 * e + 3] * inv);
                 } else {
                     // through shared memory (Q's rows of this warp, which no product needs any more), so
                     // that a store writes whole lines: piece e of row lane lies at e ^ (lane % 8)

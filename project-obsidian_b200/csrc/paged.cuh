@@ -177,8 +177,9 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 // ---- rows whose result is not finite although the sum of their exponentials is: a NaN
 // or an infinity in V, which the products spread to rows that do not see it (0 * NaN) and
 // turn into NaN (infinity times what rounding left of p).  Their dimensions that are not
-// finite are computed again, 16 rows by a warp: p from the known maximum and sum, the
-// products on mma.sync with the positions that hold anything not finite taken out, and
+// finite are computed again, 16 rows by a warp: p from the known maximum and sum (divided
+// by the sum before the products: finite values that only added up past fp32 do not here),
+// the products on mma.sync with the positions that hold anything not finite taken out, and
 // those, for the rows that see them, by fp32 FMAs, where IEEE arithmetic does what the
 // formula says.
 //
@@ -186,9 +187,14 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 // holds.  One prompt of 4096 (32 / 4 heads of 128, bf16) with one infinity at its front,
 // which every row sees: 1.9 ms; with nothing but infinities in V 8.9 ms; 155 us without.
 // A row by a warp, one position at a time, took 25 ms for a prompt of 2048.
+// A part's sums and its l are kept times 2^-28: l is at most 2^20 positions times 2^8 (a
+// maximum in use that the scores have outgrown), so no join of finite values passes fp32.
+constexpr float kJoinScale = 1.0f / (1 << 28);
+static_assert(kPagedMaxLen <= 1 << 20, "l");
+
 struct AgainRows {              // a lane's two rows: g and g + 8 of 16, g = lane / 4
     const uint16_t* q[2];       // null: no such row
-    void* out[2];               // 16-bit values, or fp32 (then times l)
+    void* out[2];               // 16-bit values, or a part's fp32 sums
     int i[2], lo[2];            // its position and its window's first
     float ref[2], l[2];         // p = 2^(scale log2 e q . k - ref) / l
 };
@@ -336,7 +342,7 @@ __device__ __forceinline__ void attend_again(const PagedArgs& a, int s, int h, c
                 float* dst = static_cast<float*>(rows.out[r]) + d;
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if (!(fabsf(dst[e]) <= 3.4e38f)) dst[e] = acc[e][2 * r + b] / wl[r];
+                    if (!(fabsf(dst[e]) <= 3.4e38f)) dst[e] = acc[e][2 * r + b] * kJoinScale / wl[r];
             } else {
                 uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(rows.out[r]) + d);
                 const uint4 y = *dst;

@@ -248,3 +248,32 @@ def test_infinities_cost_a_bounded_time(torch_):
         assert bool((out[..., 9] == inf).all())
         assert bool((out == inf).all()) if every else bool(out[..., :9].isfinite().all() and out[..., 10:].isfinite().all())
     ctx.close()
+
+
+# ------------------------------------------------------- values near bf16's largest
+@pytest.mark.parametrize("heads,kv,hd,ln", [(8, 1, 128, 2), (32, 4, 128, 700), (8, 1, 64, 9000), (4, 2, 80, 130)])
+@pytest.mark.parametrize("signs", [False, True])
+def test_sums_past_fp32_of_values_that_are_not(torch_, heads, kv, hd, ln, signs):
+    """Values of 1e38 to bf16's largest: a sum of p v over some positions lies past fp32's largest number before it
+    is divided by the sum of p; the output does not."""
+    from paged_util import Cache
+    from test_gpu_paged import check_decode, check_prefill
+
+    torch = torch_
+    c = Cache([ln, 40], kv, hd, 16, "bf16", seed=112)
+    big = torch.finfo(torch.bfloat16).max
+    gen = torch.Generator(device="cuda").manual_seed(113)
+    for s, n in enumerate(c.lens):
+        j = torch.arange(n, device="cuda")
+        x = big * (0.3 + 0.7 * torch.rand((n, kv, hd), generator=gen, device="cuda"))
+        if signs:
+            x = torch.where(torch.rand(x.shape, generator=gen, device="cuda") < 0.5, -x, x)
+        x[:, :, 0] = big
+        x[:, :, 1] = 1.0 + torch.rand((n, kv), generator=gen, device="cuda")  # and an ordinary dimension
+        c.put(s, j, c.kd[s], x.to(c.dtype))
+    ctx = make_ctx(heads, kv, hd, 16, max_len=9000, weights=True)
+    check_decode(torch, c, ctx, heads, 0, 0, 112)
+    check_decode(torch, c, ctx, heads, 0, 0, 112, weights=True)
+    check_prefill(torch, c, ctx, heads, [min(ln, 3), 40], 0, 0, 112)
+    check_prefill(torch, c, ctx, heads, [min(ln, 700), 1], 0, 0, 112)
+    ctx.close()
