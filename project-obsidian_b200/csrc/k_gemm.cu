@@ -132,6 +132,7 @@ __device__ __forceinline__ bool sub_form_ok(uint32_t s_bits) {
 }
 
 // which wait timed out (recorded in the context's second error word)
+// (obs_check_device names the codes' kernel)
 enum WaitCode : int { kWtEmptyW = 11, kWtSfreeB, kWtAccEmpty, kWtAReady, kWtFullW, kWtSfreeA, kWtFullB, kWtAccFull };
 
 __device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, volatile int* abort, int code,

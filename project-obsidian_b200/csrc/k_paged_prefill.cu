@@ -90,6 +90,7 @@ struct Pf {
     static constexpr int O = 256;                     // TMEM: S of tile x, buffer b at 128 x + 64 b; O at 256 + 128 x
 };
 
+// (obs_check_device names the codes' kernel)
 enum Wait : int { kWtEmpty = 31, kWtFull, kWtQ, kWtS, kWtP, kWtPv, kWtO, kWtTurn };
 
 // mbar_wait without the suspend hint (waits here are shorter than waking up takes)

@@ -1305,8 +1305,12 @@ extern "C" int obs_check_device(obs_ctx* ctx, void* stream) {
         CU(cudaMemset(ctx->fused.ypart, 0, (size_t)kFusedMaxT * ctx->sh.K * (ctx->sh.I / kGroup) * ctx->sh.H * 8), "reset");
         CU(cudaMemset(ctx->fused.lst, 0, (size_t)4 * kFusedMaxT * ctx->sh.E * 8), "reset");
         if (flag == kDevTimeout) {
+            // the kernels' wait codes (0: a wait without one)
+            const int code = words[1];
+            const char* where = code >= 11 && code <= 18 ? "expert GEMM" : code >= 31 && code <= 38 ? "paged prefill" : nullptr;
             char msg[96];
-            snprintf(msg, sizeof msg, "a device-side wait gave up (timeout; GEMM wait code %d)", words[1]);
+            if (where) snprintf(msg, sizeof msg, "a device-side wait gave up (timeout; %s, wait code %d)", where, code);
+            else snprintf(msg, sizeof msg, "a device-side wait gave up (timeout)");
             return fail(ctx, OBS_ERR_TIMEOUT, msg);
         }
         if (flag == kDevBadTile) return fail(ctx, OBS_ERR_INVALID, "device refused a GEMM tile outside its buffers");

@@ -277,3 +277,17 @@ def test_sums_past_fp32_of_values_that_are_not(torch_, heads, kv, hd, ln, signs)
     check_prefill(torch, c, ctx, heads, [min(ln, 3), 40], 0, 0, 112)
     check_prefill(torch, c, ctx, heads, [min(ln, 700), 1], 0, 0, 112)
     ctx.close()
+
+
+# ------------------------------------------------------------------ messages
+def test_a_timeout_names_the_kernel_that_waited(torch_):
+    """A wait that ran out outside the expert GEMM (obs_probe_wait: one wait on a stamp that nothing writes, 10 ms)
+    is not reported as one of the GEMM's."""
+    ctx = obsmoe.MoeContext(obsmoe.MoeShape(2048, 256, 16, 4, n_layers=1, max_tokens=1), 0)
+    ctx.set_wait_limit(10_000_000)
+    ctx.probe_wait()
+    with pytest.raises(obsmoe.ObsError, match="gave up") as e:
+        ctx.check_device()
+    assert e.value.status == 5 and "GEMM" not in str(e.value)
+    ctx.check_device()
+    ctx.close()
