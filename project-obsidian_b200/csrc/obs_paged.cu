@@ -70,11 +70,15 @@ const char* paged_args(const PagedState* p, const obs_paged_kv* kv, int* err, Pa
     return nullptr;
 }
 
-const char* query_args(const PagedArgs& a, const void* q, int64_t q_stride, const void* out, int window, int n_sink,
-                       float scale) {
+const char* query_args(const PagedArgs& a, const void* q, int64_t q_stride, const void* out, int rows, int window,
+                       int n_sink, float scale) {
     if (!q || !out) return "null pointer";
     if (!aligned16(q) || !aligned16(out) || q_stride % 8) return "q and out must be 16-byte aligned, q_stride a multiple of 8";
-    if (q_stride < (int64_t)a.nkv * a.group * a.hd) return "q_stride is smaller than a row";
+    const int64_t row = (int64_t)a.nkv * a.group * a.hd;
+    if (q_stride < row) return "q_stride is smaller than a row";
+    // (rows that come out not finite are computed again, from q)
+    const char *qb = static_cast<const char*>(q), *ob = static_cast<const char*>(out);
+    if (ob < qb + 2 * ((rows - 1) * q_stride + row) && qb < ob + 2 * rows * row) return "out may not overlap q";
     if (window < 0 || n_sink < 0) return "window and n_sink must not be negative";
     if (!(scale >= 0.0f) || scale > 3.0e38f) return "scale must be finite and not negative (0: 1/sqrt(head_dim))";
     return nullptr;
@@ -190,7 +194,7 @@ extern "C" int obs_paged_decode(obs_ctx* ctx, const obs_paged_kv* kv, const void
                                 int window, int n_sink, float scale, float* weights, int w_stride, void* stream) {
     PAGED_BEGIN();
     if (a.n_seqs == 0) return OBS_OK;
-    if (const char* m = query_args(a, q, q_stride, out, window, n_sink, scale)) return ctx_fail(ctx, OBS_ERR_INVALID, m);
+    if (const char* m = query_args(a, q, q_stride, out, a.n_seqs, window, n_sink, scale)) return ctx_fail(ctx, OBS_ERR_INVALID, m);
     int code;
     if (const char* m = decode_args(ps, a, weights, w_stride, &code)) return ctx_fail(ctx, code, m);
     if (weights && w_stride < a.cap) a.cap = w_stride;  // a longer sequence is refused on the device
@@ -209,7 +213,7 @@ extern "C" int obs_paged_prefill(obs_ctx* ctx, const obs_paged_kv* kv, const voi
     if (T == 0) return OBS_OK;
     if (a.n_seqs == 0) return ctx_fail(ctx, OBS_ERR_INVALID, "rows without sequences");
     if (!q_start) return ctx_fail(ctx, OBS_ERR_INVALID, "null pointer");
-    if (const char* m = query_args(a, q, q_stride, out, window, n_sink, scale)) return ctx_fail(ctx, OBS_ERR_INVALID, m);
+    if (const char* m = query_args(a, q, q_stride, out, T, window, n_sink, scale)) return ctx_fail(ctx, OBS_ERR_INVALID, m);
     const float sc = scale > 0.0f ? scale : 1.0f / sqrtf((float)a.hd);
     PrefillArgs p{a, reinterpret_cast<const uint16_t*>(q), q_stride, reinterpret_cast<uint16_t*>(out), q_start, T, window,
                   n_sink, sc, sc * kLog2e, parts.wait_ns, 1, nullptr, nullptr};

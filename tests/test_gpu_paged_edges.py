@@ -291,3 +291,26 @@ def test_a_timeout_names_the_kernel_that_waited(torch_):
     assert e.value.status == 5 and "GEMM" not in str(e.value)
     ctx.check_device()
     ctx.close()
+
+
+def test_out_may_not_overlap_q(torch_):
+    """Rows with an infinity among their values are computed again from q, which must still be there."""
+    from paged_util import Cache
+
+    torch = torch_
+    c = Cache([30, 40, 50], 2, 64, 16, "bf16", seed=150)
+    ctx = make_ctx(8, 2, 64, 16, seqs=3, max_len=64)
+    start = torch.tensor([0, 1, 2, 3], dtype=torch.int32, device="cuda")
+    pool = queries(torch, 12, 8, 64, c.dtype, 150)
+    for q, out in ((pool[:3], pool[:3]), (pool[:3], pool[2:5]), (pool[4:7], pool[2:5]), (pool[::4], pool[6:9])):
+        with pytest.raises(obsmoe.ObsError, match="overlap"):
+            ctx.paged_decode(view(c), q, out)
+        with pytest.raises(obsmoe.ObsError, match="overlap"):
+            ctx.paged_prefill(view(c), q, out, start, 3)
+    want = torch.empty_like(pool[:3])
+    for q, out in ((pool[:3], pool[3:6]), (pool[9:], pool[6:9])):
+        ctx.paged_decode(view(c), q, out)
+        ctx.paged_decode(view(c), q, want)
+        ctx.check_device()
+        assert torch.equal(out, want)
+    ctx.close()
