@@ -47,14 +47,15 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 // The caller's cache against the context's configuration; fills *a or returns a message.
 const char* paged_args(const PagedState* p, const obs_paged_kv* kv, int* err, PagedArgs* a) {
-    if (!kv || !kv->k || !kv->v || !kv->block_table || !kv->kv_len) return "null cache pointer";
+    // (no sequences: a table and lengths of no elements have no address)
+    if (!kv || !kv->k || !kv->v || (kv->n_seqs != 0 && (!kv->block_table || !kv->kv_len))) return "null cache pointer";
     const obs_paged_config& c = p->cfg;
     if (!aligned16(kv->k) || !aligned16(kv->v)) return "k and v must be 16-byte aligned";
     if (kv->page_stride % 8 || kv->slot_stride % 8 || kv->head_stride % 8)
         return "cache strides must be multiples of 8 elements (16 bytes)";
     if (kv->page_stride < 0 || kv->slot_stride < 0 || kv->head_stride < 0) return "cache strides must not be negative";
     if (kv->n_seqs < 0 || kv->n_seqs > c.max_seqs) return "n_seqs out of range (0..max_seqs)";
-    if (kv->n_pages <= 0 || kv->table_pages <= 0) return "n_pages and table_pages must be positive";
+    if (kv->n_pages <= 0 || kv->table_pages < 0 || (kv->n_seqs > 0 && kv->table_pages == 0)) return "n_pages and table_pages must be positive";
     if (kv->n_seqs > 1 && kv->table_stride < kv->table_pages) return "table_stride is smaller than table_pages";
     const int64_t room = (int64_t)kv->table_pages * c.page_size;
     a->k = reinterpret_cast<const uint16_t*>(kv->k);
@@ -228,6 +229,7 @@ extern "C" int obs_paged_evict(obs_ctx* ctx, const obs_paged_kv* kv, const obs_p
     PagedArgs d{};
     if (const char* m = paged_args(ps, dst, parts.err, &d)) return ctx_fail(ctx, OBS_ERR_INVALID, m);
     if (d.n_seqs != a.n_seqs) return ctx_fail(ctx, OBS_ERR_INVALID, "dst has another number of sequences");
+    if (a.n_seqs == 0) return OBS_OK;
     if (!weights || !kept || !new_len) return ctx_fail(ctx, OBS_ERR_INVALID, "null pointer");
     if (budget <= 0 || n_sink < 0 || n_recent < 0 || (int64_t)n_sink + n_recent > budget)
         return ctx_fail(ctx, OBS_ERR_INVALID, "need 0 <= n_sink + n_recent <= budget and budget > 0");
@@ -235,7 +237,6 @@ extern "C" int obs_paged_evict(obs_ctx* ctx, const obs_paged_kv* kv, const obs_p
     if (w_stride <= 0 || (weights_dst && w_stride < budget))
         return ctx_fail(ctx, OBS_ERR_INVALID, "w_stride must be positive (and at least budget with weights_dst)");
     if (new_len == kv->kv_len) return ctx_fail(ctx, OBS_ERR_INVALID, "new_len may not alias kv_len");
-    if (a.n_seqs == 0) return OBS_OK;
     if (w_stride < a.cap) a.cap = w_stride;  // a longer sequence is refused on the device
     return launched(ctx,
                     launch_paged_evict(a, d, weights, weights_dst, w_stride, budget, n_sink, n_recent, kept, new_len,

@@ -314,3 +314,23 @@ def test_out_may_not_overlap_q(torch_):
         ctx.check_device()
         assert torch.equal(out, want)
     ctx.close()
+
+
+def test_no_sequences(torch_):
+    """A batch of no sequences: tensors of no elements (no address), nothing to do."""
+    torch = torch_
+    ctx = make_ctx(8, 2, 64, 16, seqs=3, max_len=64, weights=True)
+    k, v = (torch.full((4, 16, 2, 64), 0.5, dtype=torch.bfloat16, device="cuda") for _ in "kv")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    for pages in (4, 0):
+        kv = obsmoe.PagedKV(k, v, torch.empty((0, pages), **i32), torch.empty(0, **i32))
+        q, rows, w = torch.empty((0, 8, 64), dtype=k.dtype, device="cuda"), k[:0, 0], torch.empty((0, 2, 64), device="cuda")
+        none = torch.empty(0, **i32)
+        ctx.paged_append(kv, rows, rows, none, none, 0)
+        ctx.paged_decode(kv, q, q.clone())
+        ctx.paged_decode(kv, q, q.clone(), weights=w)
+        ctx.paged_prefill(kv, q, q.clone(), torch.zeros(1, **i32), 0)
+        ctx.paged_evict(kv, kv, w, w, 32, kept=torch.empty((0, 2, 32), **i32), new_len=torch.empty(0, **i32))
+        ctx.check_device()
+    assert bool((k == 0.5).all()) and bool((v == 0.5).all())
+    ctx.close()
