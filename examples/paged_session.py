@@ -32,10 +32,11 @@ def quantised(rng, rows, cols):
 
 
 def make_model(n_layers, max_tokens, max_seq, n_seqs, seed=0):
-    """A context with every layer's experts, attention and the model's ends."""
+    """A context with every layer's experts, attention and the model's ends.  Its n_seqs sequences live in the
+    session's pages: no dense caches.  max_seq: RoPE's positions, which go on after an eviction."""
     rng = np.random.default_rng(seed)
     ctx = obsmoe.MoeContext(obsmoe.MoeShape(H, INTER, EXPERTS, TOP_K, n_layers=n_layers, max_tokens=max_tokens))
-    ctx.attn_init(HEADS, KV_HEADS, HEAD_DIM, max_seq, n_seqs)
+    ctx.attn_init(HEADS, KV_HEADS, HEAD_DIM, max_seq, n_seqs=0)
     ones = np.full(H, 0x3F80, np.uint16)
     for layer in range(n_layers):
         ctx.synth_layer(layer, seed)

@@ -107,7 +107,7 @@ typedef struct obs_attn_config {
     int32_t n_kv_heads;  /* key/value heads (4); n_heads a multiple of it, at most 8 times it */
     int32_t head_dim;    /* <= 128, a multiple of 8; n_heads * head_dim a multiple of 2048 */
     int32_t max_seq;     /* positions per cache (<= 40960) */
-    int32_t n_seqs;      /* sequences (caches) per layer */
+    int32_t n_seqs;      /* sequences (caches) per layer; 0: no dense caches, for obs_paged_attn_forward alone */
     float rope_theta;    /* 1e7 */
 } obs_attn_config;
 
@@ -289,7 +289,8 @@ int obs_paged_evict(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_kv* ds
  * token t is sequence t's; weights optional) or obs_paged_prefill (q_start as
  * there), the o projection and the residual.  kv->kv_len already counts this call's
  * tokens.  Needs obs_attn_init, obs_load_attn and obs_paged_init of the same heads
- * and head_dim in bf16; the dense caches are not used.  pos[t] is below
+ * and head_dim in bf16; the dense caches are not used (obs_attn_config.n_seqs may be
+ * 0).  pos[t] is below
  * obs_attn_config.max_seq (<= 40960), the RoPE table's end, however long the cache may
  * be and however much of it has been evicted: a token beyond it, or one with a sequence
  * or slot outside the cache, is refused on the device (OBS_ERR_INVALID from

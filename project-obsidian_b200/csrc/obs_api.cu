@@ -565,17 +565,17 @@ extern "C" int obs_attn_init(obs_ctx* ctx, const obs_attn_config* ac) {
     if (!ctx->attn.empty()) return fail(ctx, OBS_ERR_STATE, "attention already initialised");
     const int nq = ac->n_heads, nkv = ac->n_kv_heads, hd = ac->head_dim;
     if (nq <= 0 || nkv <= 0 || nq % nkv || nq / nkv > 8 || hd <= 0 || hd > 128 || hd % 8 || (nq * hd) % 2048 ||
-        ac->max_seq <= 0 || ac->max_seq > kAttnMaxSeq || ac->n_seqs <= 0 || !(ac->rope_theta > 0.0f))
+        ac->max_seq <= 0 || ac->max_seq > kAttnMaxSeq || ac->n_seqs < 0 || !(ac->rope_theta > 0.0f))
         return fail(ctx, OBS_ERR_INVALID,
                     "bad attention config (heads a multiple of kv heads, at most 8 per kv head, head_dim <= 128 "
-                    "a multiple of 8, heads*head_dim a multiple of 2048, 0 < max_seq <= 40960, n_seqs > 0, "
+                    "a multiple of 8, heads*head_dim a multiple of 2048, 0 < max_seq <= 40960, n_seqs >= 0, "
                     "rope_theta > 0)");
     CU(cudaSetDevice(ctx->device), "cudaSetDevice");
     ctx->acfg = *ac;
     const int T = ctx->cfg.max_tokens, H = ctx->sh.H, W = (nq + 2 * nkv) * hd;
     const size_t sizes[] = {(size_t)ac->max_seq * hd * 4, (size_t)T * W * 4, (size_t)T * H * 2, (size_t)T * nq * hd * 2,
                             (size_t)T * nq * hd * 2, (size_t)T * H * 4,
-                            sdpa_part_floats(T, nq, nkv, hd, ctx->num_sms) * 4, (size_t)T * nkv * hd * 4};
+                            ac->n_seqs ? sdpa_part_floats(T, nq, nkv, hd, ctx->num_sms) * 4 : 0, (size_t)T * nkv * hd * 4};
     size_t total = 0;
     for (size_t sz : sizes) total += align_up(sz, 256);
     CU(cudaMalloc(&ctx->attn_scratch, total), "attention scratch");
@@ -616,8 +616,10 @@ extern "C" int obs_load_attn(obs_ctx* ctx, int layer, const obs_attn_weights* w,
                          (void**)&L.o_b,   (void**)&L.in_norm, (void**)&L.q_norm, (void**)&L.k_norm, (void**)&L.kc,
                          (void**)&L.vc};
         for (int i = 0; i < 11; ++i) *ptrs[i] = p, p += align_up(sizes[i], 256);
-        CU(cudaMemset(L.kc, 0, cache), "cache init");
-        CU(cudaMemset(L.vc, 0, cache), "cache init");
+        if (cache) {
+            CU(cudaMemset(L.kc, 0, cache), "cache init");
+            CU(cudaMemset(L.vc, 0, cache), "cache init");
+        }
     }
     const cudaMemcpyKind kind = src_on_device ? cudaMemcpyDeviceToDevice : cudaMemcpyHostToDevice;
     const size_t wq = rq * (H / 8) * 4, wk = rk * (H / 8) * 4, gq = rq * (H / 64) * 2, gk = rk * (H / 64) * 2;
@@ -649,6 +651,7 @@ extern "C" int obs_attn_forward(obs_ctx* ctx, int layer, const uint16_t* x, uint
     if (ctx->attn.empty()) return fail(ctx, OBS_ERR_STATE, "attention not initialised (obs_attn_init)");
     if (layer < 0 || layer >= (int)ctx->attn.size()) return fail(ctx, OBS_ERR_INVALID, "layer out of range");
     if (!ctx->attn[layer].loaded) return fail(ctx, OBS_ERR_STATE, "attention layer not loaded");
+    if (ctx->acfg.n_seqs == 0) return fail(ctx, OBS_ERR_STATE, "no dense caches (obs_attn_init with n_seqs 0)");
     if (T < 0 || T > ctx->cfg.max_tokens) return fail(ctx, OBS_ERR_INVALID, "T out of range (0..max_tokens)");
     if (T == 0) return OBS_OK;
     if (!x || !out || !seq || !pos) return fail(ctx, OBS_ERR_INVALID, "null pointer");

@@ -334,3 +334,42 @@ def test_no_sequences(torch_):
         ctx.check_device()
     assert bool((k == 0.5).all()) and bool((v == 0.5).all())
     ctx.close()
+
+
+# --------------------------------------------------- the attention block without dense caches
+def test_attention_block_without_dense_caches(torch_):
+    """obs_attn_init with n_seqs 0: the paged block gives the same bits, the dense entry points refuse, and the
+    caches' memory is not taken."""
+    import oracle as O
+    from parity_util import dev
+
+    torch = torch_
+    H, nq, nkv, hd, page, max_seq = 2048, 32, 4, 128, 16, 40960
+    A = O.synth_attn(seed=9, layer=0, H=H, nq=nq, nkv=nkv, hd=hd)
+    x = dev(torch, O.synth_x(80, 0, 5, H))
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    got, taken = [], []
+    for n_seqs in (2, 0):
+        before = torch.cuda.mem_get_info()[0]
+        ctx = obsmoe.MoeContext(obsmoe.MoeShape(H, 256, 16, 4, n_layers=1, max_tokens=8), 0)
+        ctx.attn_init(nq, nkv, hd, max_seq, n_seqs, 1e7)
+        ctx.load_attn(0, A)
+        ctx.paged_init(nq, nkv, hd, page, max_seqs=2, max_kv_len=64)
+        taken.append(before - torch.cuda.mem_get_info()[0])
+        k, v = (torch.zeros((8, page, nkv, hd), dtype=torch.bfloat16, device="cuda") for _ in "kv")
+        kv = obsmoe.PagedKV(k, v, torch.arange(8, dtype=torch.int32, device="cuda").reshape(2, 4), i32(3, 2))
+        y = torch.empty_like(x)
+        ctx.paged_attn_forward(0, kv, x, y, 5, i32(0, 0, 0, 1, 1), i32(0, 1, 2, 7, 40959), i32(0, 1, 2, 0, 1), i32(0, 3, 5))
+        ctx.check_device()
+        got.append((y, k.view(torch.int16), v.view(torch.int16)))
+        if n_seqs == 0:
+            with pytest.raises(obsmoe.ObsError, match="no dense caches"):
+                ctx.attn_forward(0, x, torch.empty_like(x), 1, i32(0), i32(0))
+            with pytest.raises(obsmoe.ObsError, match="out of bounds"):
+                ctx.kv_read(0, 0, 0, 1, k)
+        ctx.close()
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    assert taken[0] - taken[1] >= 2 * 2 * nkv * max_seq * hd * 2
+    with pytest.raises(obsmoe.ObsError, match="bad attention config"):
+        ctx = obsmoe.MoeContext(obsmoe.MoeShape(H, 256, 16, 4, n_layers=1, max_tokens=8), 0)
+        ctx.attn_init(nq, nkv, hd, 64, -1, 1e7)
