@@ -373,3 +373,36 @@ def test_attention_block_without_dense_caches(torch_):
     with pytest.raises(obsmoe.ObsError, match="bad attention config"):
         ctx = obsmoe.MoeContext(obsmoe.MoeShape(H, 256, 16, 4, n_layers=1, max_tokens=8), 0)
         ctx.attn_init(nq, nkv, hd, 64, -1, 1e7)
+
+
+# ----------------------------------------------------------- pages at every position
+@pytest.mark.parametrize("page", [1, 3, 16, 63, 64, 1000, 1023, 1024])
+def test_every_position_of_the_longest_sequence_lies_in_its_page(torch_, page):
+    """append to each of 2^20 positions, in a mixed order; each row is where j / page and j % page say.  A decode
+    over a window of one reads the last back."""
+    torch = torch_
+    n, hd = 1 << 20, 8
+    pages = -(-n // page)
+    gen = torch.Generator(device="cuda").manual_seed(page)
+    table = torch.randperm(pages, generator=gen, device="cuda").to(torch.int32)[None]
+    k, v = (torch.zeros((pages, page, 1, hd), dtype=torch.bfloat16, device="cuda") for _ in "kv")
+    slot = torch.randperm(n, generator=gen, device="cuda").to(torch.int32)
+    # the position in three digits of 7 bits, which bf16 holds
+    digits = torch.stack([slot >> s & 127 for s in (0, 7, 14)] + [slot * 0 + 1] * 5, dim=1).to(torch.bfloat16)
+    ctx = make_ctx(1, 1, hd, page, seqs=1, max_len=n)
+    length = torch.tensor([n], dtype=torch.int32, device="cuda")
+    kv = obsmoe.PagedKV(k, v, table, length)
+    ctx.paged_append(kv, digits.view(n, 1, hd), (-digits).view(n, 1, hd), torch.zeros_like(slot), slot, n)
+    ctx.check_device()
+    j = torch.arange(n, device="cuda")
+    want = torch.stack([j >> s & 127 for s in (0, 7, 14)] + [j * 0 + 1] * 5, dim=1).to(torch.bfloat16)
+    p, o = table[0].long()[j // page], j % page
+    assert torch.equal(k[p, o, 0], want) and torch.equal(v[p, o, 0], -want)
+    q = torch.ones((1, 1, hd), dtype=torch.bfloat16, device="cuda")
+    for last in (n, n - 1, page, page + 1, 1, n // 2 + 1):
+        length.fill_(last)
+        out = torch.empty_like(q)
+        ctx.paged_decode(kv, q, out, window=1)
+        ctx.check_device()
+        assert torch.equal(out[0, 0], -want[last - 1]), last
+    ctx.close()
