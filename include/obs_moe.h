@@ -255,10 +255,11 @@ int obs_paged_append(obs_ctx* ctx, const obs_paged_kv* kv, const void* k, const 
  * q_stride elements apart) at position i = kv_len[s] - 1 sees the positions j <= i
  * with window == 0 or i - j < window or j < n_sink;
  *   out[s][h] = sum_j p_j v_j,  p = softmax_j(scale * q . k_j)   (scale 0: 1/sqrt(head_dim))
- * out [n_seqs][n_heads][head_dim], not overlapping q.  A sequence of length 0 gives zeros.  Sums and
- * the softmax in fp32, one rounding at the end (p is rounded to the element type
- * for the product with v).  weights (optional, fp32 [n_seqs][n_kv_heads][w_stride]):
- * weights[s][g][j] += the p_j of KV head g's query heads, summed. */
+ * out [n_seqs][n_heads][head_dim], not overlapping q.  A sequence of length 0 gives
+ * zeros.  Sums and the softmax in fp32, one rounding at the end (p goes into the product
+ * with v as two values of the element type, its rounding and the rest).  weights
+ * (optional, fp32 [n_seqs][n_kv_heads][w_stride]): weights[s][g][j] += the p_j of KV head
+ * g's query heads, summed. */
 int obs_paged_decode(obs_ctx* ctx, const obs_paged_kv* kv, const void* q, int64_t q_stride, void* out, int window,
                      int n_sink, float scale, float* weights, int w_stride, void* stream);
 /* Attention of the new tokens of several prompts (or chunks of them): rows
@@ -266,7 +267,10 @@ int obs_paged_decode(obs_ctx* ctx, const obs_paged_kv* kv, const void* q, int64_
  * T, not decreasing) are sequence s's last positions, the last of them kv_len[s] - 1
  * (their keys and values already appended); each sees what a decode at its position
  * would see.  A row with nothing to see (more rows than kv_len[s]) gives zeros.  out does
- * not overlap q. */
+ * not overlap q.  As decode, but p is rounded to the element type once where 512
+ * positions or more are seen: up to 40% on top of the output's own rounding error (rms).
+ * Prompts add nothing to the weights that obs_paged_evict goes by: before the first decode
+ * steps with weights, a prompt's positions all have what the caller put there. */
 int obs_paged_prefill(obs_ctx* ctx, const obs_paged_kv* kv, const void* q, int64_t q_stride, void* out,
                       const int32_t* q_start, int T, int window, int n_sink, float scale, void* stream);
 /* Eviction by accumulated attention weight, per sequence and KV head: of n =

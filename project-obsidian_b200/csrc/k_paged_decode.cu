@@ -4,7 +4,7 @@
 //   out[s][h] = sum_j p_j v_j,  p = softmax over the visible j of scale * q[s][h] . k_j
 //
 // What bounds it: every visible row of K and V is read once from memory for the
-// group of query heads that share it, 4 * head_dim * 2 bytes against 4 * head_dim *
+// group of query heads that share it, 2 * head_dim * 2 bytes against 4 * head_dim *
 // group operations, 8 operations a byte at a group of 8: far below what the tensor
 // cores want and, with the conversions to fp32, above what the FMA units give, so
 // the two products run on mma.sync tiles whose N is the group (tcgen05's M = 128
@@ -27,9 +27,9 @@
 // not depend on which one that is.
 //
 // p enters the second product as two 16-bit values, its rounding and what the
-// rounding left: the tensor cores multiply 16-bit values, one rounding of p would
-// cost a short sequence (few p to average over) as much as the output's own, and
-// the second set of products is hidden behind the loads.
+// rounding left: the tensor cores multiply 16-bit values, one rounding of p would add
+// as much error as the output's own (k_paged_prefill.cu has the figures), and the
+// second set of products is hidden behind the loads.
 //
 // f16 holds nothing below 2^-25, and a first position that many scores fall 2^25 behind
 // is common: p <= 1 is multiplied by 2^15 there, and the sums by 2^-15 at their end.
@@ -39,9 +39,9 @@
 // (attend_again), before the join.  When nothing is wrong this costs a comparison.
 //
 // Measured, 32 / 4 heads of 128: 32 sequences of 61 to 32768 positions in f16, pages of
-// 16: 172 us, 6.5 TB/s, 97% of the measured copy rate; 128 sequences with a window of
-// 1024 and 4 sinks 52 us (79%: each CTA starts and ends inside some item, and joining
-// takes it from loading); one of 2049 9.6 us, where the launch, four dependent accesses
+// 16: 173 to 190 us on different GPUs, 6.4 to 5.9 TB/s, 98% to 89% of the measured copy
+// rate; 128 sequences with a window of 1024 and 4 sinks 52 to 57 us (79% to 72%: each CTA
+// starts and ends inside some item, and joining takes it from loading); one of 2049 9.4 us, where the launch, four dependent accesses
 // to the first rows and the join are nearly all of it.
 #include "paged.cuh"
 

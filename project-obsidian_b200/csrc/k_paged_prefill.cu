@@ -24,7 +24,7 @@
 // Sixteen warps:
 //   0-3, 4-7   softmax of row tile A, of B: running maximum m and sum l of the thread's
 //              row.  O is rescaled only when the maximum has grown by more than 2^8 (p
-//              stays below 2^8, far inside both types), by the same threads, between a
+//              stays below 2^8, in f16 below 2^15), by the same threads, between a
 //              tile's S and its P, when no product touches O.  The two row tiles' warps
 //              of one scheduler take turns at the exponentials: in step they would share
 //              the exponential unit and then leave it idle, and both row tiles' products
@@ -37,8 +37,8 @@
 //              the tensor cores see them is the issuing warp's (in the loading warps it
 //              would wait for every load in flight)
 // Measured for 32 / 4 heads of 128 in bf16: one prompt of 4096 137 us, 1.0 PFLOP/s, 60% of
-// the measured bf16 rate (up to 154 us, 53%, with the clock under its power limit); one
-// of 8192 with a window of 1024 and 4 sinks 177 us, 730 TFLOP/s.  What bounds it: a tile
+// the measured bf16 rate (up to 158 us, 52%, with the clock under its power limit); one
+// of 8192 with a window of 1024 and 4 sinks 173 to 184 us, 750 to 703 TFLOP/s.  What bounds it: a tile
 // takes 1770 cycles a block, of which the exponentials (64 a row at 16 a clock and SM)
 // need 1024 and the products 1370 (390 for a 128 x 64 x 128 QK, whose operands come from
 // shared memory at its full rate, 294 for a PV); half the products left out saves 5%,
@@ -46,11 +46,17 @@
 // A block's start (finding it, Q, the first tiles) and end cost 9000 cycles, a fifth of
 // a window of 1024.
 //
-// p is rounded to 16 bits once; over many positions the roundings average out far
-// below the output's own.  Where a row of the block sees fewer than kFewKeys
-// positions they do not, and what the rounding left is multiplied too (the other
-// half of S's columns holds it): half as much work again for the first tiles of a
-// prompt.
+// p is rounded to 16 bits once.  Against sum p |v| the roundings average out with the
+// square root of the number of positions; against the output of values without a common
+// mean, which shrinks the same way, they do not: rms error of unit normal inputs against
+// 64 bits 2.2e-3 to 2.3e-3 in bf16 from 512 to 16,432 positions where the output's own
+// rounding is 1.66e-3 (f16 2.9e-4 and 2.1e-4).  Multiplying what the rounding left too (the
+// other half of S's columns holds it) brings the error down to the output's own and
+// takes half the products again: a prompt of 4096 194 us instead of 156 us, 8192 with a
+// window 224 instead of 184, 48 rows after 16384 36.4 instead of 33.0.  So only blocks do
+// it of which a row sees fewer than kFewKeys positions, where one p can be most of the
+// sum and its rounding of the order of sum p |v| itself: the first tiles of a prompt,
+// which are few (9 prompts of 1 to 700: 30.5 us, 28.7 us without; 4096: no difference).
 //
 // f16 holds nothing below 2^-25, and a first position that many scores fall 2^25 behind
 // is common: there p is 2^7 times as large (2^15 at most, with what the maximum may have

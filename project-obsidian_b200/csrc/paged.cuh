@@ -134,18 +134,14 @@ template <int DT>
 struct Elem;
 template <>
 struct Elem<0> {
-    static __device__ __forceinline__ float f(uint16_t h) { return bf2f(h); }
     static __device__ __forceinline__ float lo(uint32_t w) { return __uint_as_float(w << 16); }
     static __device__ __forceinline__ float hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
-    static __device__ __forceinline__ uint16_t h(float f) { return f2bf(f); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf2(a, b); }
 };
 template <>
 struct Elem<1> {
-    static __device__ __forceinline__ float f(uint16_t h) { return __half2float(__ushort_as_half(h)); }
-    static __device__ __forceinline__ float lo(uint32_t w) { return f((uint16_t)w); }
-    static __device__ __forceinline__ float hi(uint32_t w) { return f((uint16_t)(w >> 16)); }
-    static __device__ __forceinline__ uint16_t h(float f) { return __half_as_ushort(__float2half_rn(f)); }
+    static __device__ __forceinline__ float lo(uint32_t w) { return __half2float(__ushort_as_half((uint16_t)w)); }
+    static __device__ __forceinline__ float hi(uint32_t w) { return __half2float(__ushort_as_half((uint16_t)(w >> 16))); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const __half2 v = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&v);
