@@ -241,7 +241,9 @@ int obs_kv_read(obs_ctx* ctx, int layer, int seq, int pos0, int n, uint16_t* k, 
  * read or written (such rows count as zeros, such a length as the largest) and
  * obs_check_device reports OBS_ERR_INVALID.
  *
- * A call over no sequences (n_seqs 0) does nothing.
+ * A call over no sequences (n_seqs 0) does nothing.  The workspace is the context's:
+ * its paged calls run one after another (on one stream, or on streams ordered by
+ * events); contexts are independent of one another.
  * obs_paged_init: the shape that the calls below take and their workspace, once
  * per context (independent of obs_attn_init and of the number of layers). */
 int obs_paged_init(obs_ctx* ctx, const obs_paged_config* cfg);

@@ -406,3 +406,92 @@ def test_every_position_of_the_longest_sequence_lies_in_its_page(torch_, page):
         ctx.check_device()
         assert torch.equal(out[0, 0], -want[last - 1]), last
     ctx.close()
+
+
+# ------------------------------------------------------------- eviction's mixed forms
+@pytest.mark.parametrize("form", ["other pages of the same pools", "weights in place", "weights elsewhere", "no weights"])
+def test_evict_mixed_forms(torch_, form):
+    """Other pages of the same pools; rows to other pages with the weights in place; rows in place with the weights
+    to another tensor or nowhere."""
+    from paged_util import Cache
+    from test_gpu_paged import check_evicted, weights_of
+
+    torch = torch_
+    kv, hd, page, lens, budget, sinks, recent = 2, 64, 16, [700, 90, 33], 65, 3, 20
+    per = -(-budget // page)
+    c = Cache(lens, kv, hd, page, "bf16", seed=160, pages_extra=len(lens) * per)
+    ctx = make_ctx(4 * kv, kv, hd, page, max_len=max(lens))
+    w = weights_of(torch, "ties", (len(lens), kv, max(lens)), 160)
+    before = [tuple(x.clone() for x in c.rows(s, ln)) for s, ln in enumerate(lens)]
+    i32 = dict(dtype=torch.int32, device="cuda")
+    kept, new_len = torch.empty((len(lens), kv, budget), **i32), torch.empty(len(lens), **i32)
+    held = {int(p) for s, ln in enumerate(lens) for p in c.table[s, :-(-ln // page)].tolist()}
+    spare = torch.tensor([p for p in range(c.k.shape[0]) if p not in held], **i32)
+    k, v, table, w_src, w_dst = c.k, c.v, c.table, w.clone(), torch.full_like(w, 9.0)
+    if form == "other pages of the same pools":
+        table = spare[:len(lens) * per].view(len(lens), per)
+    elif form == "weights in place":
+        k, v = torch.zeros_like(c.k), torch.zeros_like(c.v)
+        w_dst = w_src
+    elif form == "no weights":
+        w_dst = None
+    ctx.paged_evict(view(c), obsmoe.PagedKV(k, v, table, new_len), w_src, w_dst, budget, n_sink=sinks, n_recent=recent, kept=kept,
+                    new_len=new_len)
+    ctx.check_device()
+    check_evicted(torch, c, before, w, kept, new_len, budget, sinks, recent, k, v, table, w_dst)
+    if form in ("other pages of the same pools", "weights in place"):  # the source stays
+        for s, ln in enumerate(lens):
+            assert all(torch.equal(a, b) for a, b in zip(before[s], c.rows(s, ln)))
+    if w_dst is not w_src:
+        assert torch.equal(w_src.view(torch.int32), w.view(torch.int32))
+    ctx.close()
+
+
+def test_a_captured_step_serves_other_lengths(torch_):
+    """append, prefill and evict in one graph on a side stream; replayed with other rows, lengths and row ranges."""
+    from paged_util import Cache
+    from test_gpu_paged import weights_of
+
+    torch = torch_
+    T, heads, kv, hd, page, budget = 60, 8, 2, 64, 16, 40
+    c = Cache([200, 90, 130], kv, hd, page, "bf16", seed=170)
+    ctx = make_ctx(heads, kv, hd, page)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    w = weights_of(torch, "plain", (3, kv, 200), 170)
+    rows, q = queries(torch, T, 2 * kv, hd, c.dtype, 170), queries(torch, T, heads, hd, c.dtype, 171)
+    k, v = rows[:, :kv].contiguous(), rows[:, kv:].contiguous()
+    seq, slot, start = torch.zeros(T, **i32), torch.zeros(T, **i32), torch.zeros(4, **i32)
+    out, kept, new_len = torch.empty_like(q), torch.empty((3, kv, budget), **i32), torch.empty(3, **i32)
+    per = -(-budget // page)
+    to = [torch.zeros((3 * per, page, kv, hd), dtype=c.dtype, device="cuda") for _ in "kv"]
+    w2, kv_ = torch.empty_like(w), view(c)
+    dst = obsmoe.PagedKV(*to, torch.arange(3 * per, **i32).view(3, per), new_len)
+
+    def step(stream=None):
+        ctx.paged_append(kv_, k, v, seq, slot, T, stream=stream)
+        ctx.paged_prefill(kv_, q, out, start, T, window=50, n_sink=2, stream=stream)
+        ctx.paged_evict(kv_, dst, w, w2, budget, n_sink=2, n_recent=9, kept=kept, new_len=new_len, stream=stream)
+
+    def results():
+        ctx.check_device()
+        r = [t.clone() for t in (out, kept, new_len, *to, w2)]
+        for t in (out, kept, new_len, *to, w2):
+            t.zero_()
+        return r
+
+    side, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    for counts, lens in (([20, 30, 10], [200, 90, 130]), ([0, 59, 1], [1, 77, 129]), ([60, 0, 0], [60, 0, 41])):
+        seq.copy_(torch.repeat_interleave(torch.arange(3), torch.tensor(counts)))
+        slot.copy_(torch.cat([torch.arange(n - m, n) for n, m in zip(lens, counts)]))
+        start.copy_(torch.tensor(np.concatenate([[0], np.cumsum(counts)])))
+        c.len.copy_(torch.tensor(lens))
+        step()
+        want = results()
+        if lens[0] == 200:
+            torch.cuda.synchronize()
+            with torch.cuda.graph(g, stream=side):
+                step(side)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(want, results()))
+    ctx.close()
