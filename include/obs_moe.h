@@ -268,7 +268,9 @@ int obs_paged_decode(obs_ctx* ctx, const obs_paged_kv* kv, const void* q, int64_
  * q_start[s] .. q_start[s+1] - 1 of q and out (device int32 [n_seqs + 1], from 0 to
  * T, not decreasing) are sequence s's last positions, the last of them kv_len[s] - 1
  * (their keys and values already appended); each sees what a decode at its position
- * would see.  A row with nothing to see (more rows than kv_len[s]) gives zeros.  out does
+ * would see.  A row with nothing to see (more rows than kv_len[s]) gives zeros; where
+ * q_start is refused (OBS_ERR_INVALID from obs_check_device), rows of no sequence are not
+ * written, and what obs_paged_attn_forward makes of them means nothing.  out does
  * not overlap q.  As decode, but p is rounded to the element type once where 512
  * positions or more are seen: up to 40% on top of the output's own rounding error (rms).
  * Prompts add nothing to the weights that obs_paged_evict goes by: before the first decode
